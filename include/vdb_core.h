@@ -409,6 +409,85 @@ int vdb_topk_merge_keyed_strided_dev(const float* d_dist, const int64_t* d_key, 
                                      int64_t list_stride_dist, int64_t list_stride_key_row, int n_lists, int nq, int k,
                                      float* d_out_dist, int64_t* d_out_row, void* stream);
 
+/* ---- operators on row tables and score rows -------------------------------------
+ * No counterpart in the reference.  A table is a matrix of rows (the vectors of a collection, or the embeddings a
+ * model learns); a score row holds one value per row of a table (what vdb_flat_distances computes for a query, or a
+ * model's logits).  The operators train such rows and answer with them: rows by number and the gradient of that,
+ * a score row's divergence from a teacher's top scores (the lists a search returns) and its gradient, one row number
+ * drawn from each score row.
+ *
+ * All take DEVICE pointers and the stream to enqueue on (NULL = the null stream), never synchronise and never
+ * allocate, so they can be captured into a graph; what they need beside inputs and outputs is the caller's `d_work`
+ * of at least the bytes that the *_workspace function names, which holds nothing between calls (two calls that may
+ * overlap take two).  Values are fp32, bf16 or fp16 (vdb_value_type); products and sums are taken in 32 bits or
+ * more and rounded once.  Rows of a matrix are contiguous and `ld` elements apart (0 for an input = one row for
+ * all); no alignment beyond the type's own is asked for.  Results do not depend on timing: equal inputs give equal
+ * bits.  n = 0 is allowed and does nothing. */
+enum vdb_value_type { VDB_VALUE_F32 = 0, VDB_VALUE_BF16 = 1, VDB_VALUE_F16 = 2 };
+
+/* out[i] = scale * table[rows[i]], i < n; a row number outside [0, n_rows) (the -1 of an unfilled result slot)
+ * gives a row of zeros.  n_rows and n below 2^31. */
+int vdb_lookup_dev(const void* d_table, int table_type, int64_t n_rows, int dim, int64_t ld, const int64_t* d_rows, int64_t n,
+                   float scale, void* d_out, int out_type, int64_t ld_out, void* stream);
+/* the same from the rows resident in a handle (fp32 or bf16 storage) */
+int vdb_rows_lookup_dev(vdb_rows* h, const int64_t* d_rows, int64_t n, float scale, void* d_out, int out_type, int64_t ld_out,
+                        void* stream);
+/* Gradient of a lookup: table_grad[r] = scale * sum of grad[i] over the i with rows[i] == r, zero for rows nobody
+ * looked up; with `accumulate` that is added to what table_grad holds and the other rows are not touched.  Row
+ * numbers outside [0, n_rows) contribute nothing.  The positions are sorted by row number (stable) and every row is
+ * summed in fp32 in an order that depends on the row numbers alone. */
+int vdb_lookup_grad_workspace(int64_t n, int64_t n_rows, int dim, int64_t* bytes);
+int vdb_lookup_grad_dev(const void* d_grad, int grad_type, int64_t ld, const int64_t* d_rows, int64_t n, float scale,
+                        void* d_table_grad, int table_type, int64_t n_rows, int dim, int64_t ld_table, int accumulate,
+                        void* d_work, int64_t work_bytes, void* stream);
+
+/* Distillation from a teacher's k best scores a row, k <= VDB_DISTILL_MAX_K: with z the `vocab` scores of a row (the
+ * student's), t_j and r_j the teacher's scores and the row numbers they belong to, tau the temperature,
+ *   q   = softmax(z / tau)
+ *   p_j = exp(t_j / tau - L), L = the log of the sum of exp(t_j / tau) over the filled slots, or teacher_lse of the
+ *         row where that is given (the teacher's mass outside the list is then left out)
+ *   loss = tau^2 * sum_j p_j (log p_j - log q_{r_j})
+ *   d loss / d z_v = tau * (sum_j p_j * q_v - sum of p_j with r_j == v)
+ * A slot with a row number outside [0, vocab) or a score of -inf is unfilled; a row without filled slots has loss
+ * and gradient 0 whatever its scores are.  stats, where wanted, takes (max z, log sum_v exp((z_v - max z) / tau)) of every
+ * row: what the gradient needs of the forward pass.  Scores of -inf have q = 0 (and loss +inf where the teacher names
+ * one); a row that holds a NaN or +inf has a NaN loss and gradient, other rows are not affected.  temperature lies in
+ * [1e-6, 1e6].
+ * The gradient of row i is scaled by grad_loss[i] (0 = zeros whatever the row holds); d_grad may be d_scores itself
+ * (same ld), otherwise the two do not overlap.  vdb_distill_step_dev computes both for weights known beforehand. */
+#define VDB_DISTILL_MAX_K 1024
+int vdb_distill_workspace(int64_t n, int64_t vocab, int64_t* bytes);
+int vdb_distill_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int64_t ld, const float* d_teacher,
+                    const int64_t* d_rows, int k, int64_t ld_teacher, int64_t ld_rows, const float* d_teacher_lse, float temperature,
+                    float* d_loss, float* d_stats, void* d_work, int64_t work_bytes, void* stream);
+int vdb_distill_grad_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int64_t ld, const float* d_teacher,
+                         const int64_t* d_rows, int k, int64_t ld_teacher, int64_t ld_rows, const float* d_teacher_lse,
+                         float temperature, const float* d_stats, const float* d_grad_loss, void* d_grad, int64_t ld_grad, void* stream);
+int vdb_distill_step_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int64_t ld, const float* d_teacher,
+                         const int64_t* d_rows, int k, int64_t ld_teacher, int64_t ld_rows, const float* d_teacher_lse,
+                         float temperature, const float* d_grad_loss, float* d_loss, float* d_stats, void* d_grad, int64_t ld_grad,
+                         void* d_work, int64_t work_bytes, void* stream);
+
+/* One row number drawn from each score row.  With z the scores that can be drawn (bit v of the row's mask set, not
+ * NaN, not -inf), ordered by (z descending, v ascending), and w_v = exp((z_v - max z) / temperature), zero below 2^-40:
+ *   temperature <= 0 (or NaN)   the first of the order
+ *   top_k > 0                   the first top_k remain
+ *   top_p < 1                   of those, each whose predecessors' weights sum to less than top_p of the total (and the first)
+ *   min_p > 0                   of those, each with w_v >= min(min_p, 1)
+ * and the draw is the first remaining row, in ascending row number, at which the running sum of the weights exceeds
+ * uniform * total (the last remaining one with a weight, should none).  Where z holds +inf, those rows have weight 1 and the others none.
+ * Weights are added as multiples of 2^-s, s = min(52, 62 - ceil(log2 vocab)), so sums are exact and borders do not
+ * depend on the order of summation.  out_row = -1 and out_logp = -inf where nothing can be drawn; out_logp (may be
+ * NULL) is the log of the drawn row's share of the remaining weights.  Settings come per row (device arrays, where
+ * given) or as one value for all.  mask: packed words as everywhere (bit v % 32 of word v / 32 set = may be drawn),
+ * rows `mask_ld` words apart, 0 = one mask for all; NULL = no mask.  smaller_first != 0: the scores are distances
+ * (z = -score).  vocab <= 2^24. */
+int vdb_sample_workspace(int64_t n, int64_t vocab, int64_t* bytes);
+int vdb_sample_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int64_t ld, int smaller_first, const float* d_uniform,
+                   const float* d_temperature, float temperature, const int32_t* d_top_k, int top_k, const float* d_top_p, float top_p,
+                   const float* d_min_p, float min_p, const uint32_t* d_mask, int64_t mask_ld, int64_t* d_out_row, float* d_out_logp,
+                   void* d_work, int64_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -144,6 +144,24 @@ SIGNATURES = {
                                            C.c_void_p, C.c_void_p]),
     "vdb_topk_merge_keyed_strided_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_int64, C.c_int, C.c_int,
                                                    C.c_int, C.c_void_p, C.c_void_p, C.c_void_p]),
+    "vdb_lookup_dev": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_float, C.c_void_p,
+                                 C.c_int, C.c_int64, C.c_void_p]),
+    "vdb_rows_lookup_dev": (C.c_int, [C.c_void_p, C.c_void_p, C.c_int64, C.c_float, C.c_void_p, C.c_int, C.c_int64, C.c_void_p]),
+    "vdb_lookup_grad_workspace": (C.c_int, [C.c_int64, C.c_int64, C.c_int, c_i64_p]),
+    "vdb_lookup_grad_dev": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_void_p, C.c_int64, C.c_float, C.c_void_p, C.c_int, C.c_int64,
+                                      C.c_int, C.c_int64, C.c_int, C.c_void_p, C.c_int64, C.c_void_p]),
+    "vdb_distill_workspace": (C.c_int, [C.c_int64, C.c_int64, c_i64_p]),
+    "vdb_distill_dev": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int64,
+                                  C.c_int64, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "vdb_distill_grad_dev": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int64,
+                                       C.c_int64, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
+    "vdb_distill_step_dev": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_void_p, C.c_void_p, C.c_int, C.c_int64,
+                                       C.c_int64, C.c_void_p, C.c_float, C.c_void_p, C.c_void_p, C.c_void_p, C.c_void_p, C.c_int64,
+                                       C.c_void_p, C.c_int64, C.c_void_p]),
+    "vdb_sample_workspace": (C.c_int, [C.c_int64, C.c_int64, c_i64_p]),
+    "vdb_sample_dev": (C.c_int, [C.c_void_p, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_void_p, C.c_void_p, C.c_float,
+                                 C.c_void_p, C.c_int, C.c_void_p, C.c_float, C.c_void_p, C.c_float, C.c_void_p, C.c_int64, C.c_void_p,
+                                 C.c_void_p, C.c_void_p, C.c_int64, C.c_void_p]),
 }
 
 _lib: Optional[C.CDLL] = None
@@ -464,6 +482,7 @@ def kmeans_accumulate(x: np.ndarray, assign_idx: np.ndarray, n_clusters: int):
 
 
 KMEANS_IVF, KMEANS_PQ = 0, 1
+DISTILL_MAX_K = 1024
 
 
 class KMeansTrainer:

@@ -1344,6 +1344,14 @@ int vdb_rows_truncate(vdb_rows* h, int64_t n) {
     return VDB_OK;
 }
 
+int vdb_rows_lookup_dev(vdb_rows* h, const int64_t* d_rows, int64_t n, float scale, void* d_out, int out_type, int64_t ld_out, void* stream) {
+    VDB_REQUIRE(h, "bad arguments to vdb_rows_lookup_dev");
+    Entry g(h);
+    const Rows& r = h->r;
+    return vdb_lookup_dev(r.bf16 ? (const void*)r.data16 : (const void*)r.data, r.bf16 ? VDB_VALUE_BF16 : VDB_VALUE_F32, r.n, r.dim,
+                          r.bf16 ? r.ld16 : r.ld, d_rows, n, scale, d_out, out_type, ld_out, stream);
+}
+
 int vdb_rows_set_prefilter(vdb_rows* h, int mode) {
     VDB_REQUIRE(h && mode >= VDB_PREFILTER_NONE && mode <= VDB_PREFILTER_AUTO, "unknown prefilter mode %d", mode);
     Entry g(h);

@@ -1,0 +1,80 @@
+// Loads and stores of fp32 / bf16 / fp16 rows for the operators on row tables and score rows: 16-byte pieces at any
+// alignment the element type allows (gfx950 reads and writes them in one instruction wherever they lie), converted to
+// fp32 and back with one rounding to nearest even.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+#include <type_traits>
+
+#include "../../include/vdb_core.h"
+
+namespace vdb {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+template <class T> struct Piece {
+    static constexpr int N = 16 / (int)sizeof(T);     // elements of one 16-byte piece
+    u32x4 raw;
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (sizeof(T) == 4) return __uint_as_float(raw[i]);
+        else if constexpr (__is_same(T, bf16_t)) return __uint_as_float((i & 1) ? (raw[i >> 1] & 0xffff0000u) : (raw[i >> 1] << 16));
+        else return (float)__builtin_bit_cast(f16_t, (uint16_t)((i & 1) ? (raw[i >> 1] >> 16) : (raw[i >> 1] & 0xffffu)));
+    }
+    __device__ __forceinline__ void set(const float* x) {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[i] = __float_as_uint(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                raw[i] = (uint32_t)__builtin_bit_cast(uint16_t, (T)x[2 * i]) | ((uint32_t)__builtin_bit_cast(uint16_t, (T)x[2 * i + 1]) << 16);
+        }
+    }
+};
+
+template <class T> __device__ __forceinline__ Piece<T> load_piece(const T* p) {
+    Piece<T> r;
+    __builtin_memcpy(&r.raw, p, 16);
+    return r;
+}
+template <class T> __device__ __forceinline__ void store_piece(T* p, const Piece<T>& v) { __builtin_memcpy(p, &v.raw, 16); }
+
+// The elements [at, at + N) of a row of `len`, those behind its end as `fill`.
+template <class T> __device__ __forceinline__ void load_values(const T* row, int64_t at, int64_t len, float fill, float* x) {
+    if (at + Piece<T>::N <= len) {
+        const Piece<T> v = load_piece(row + at);
+#pragma unroll
+        for (int i = 0; i < Piece<T>::N; ++i) x[i] = v.get(i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < Piece<T>::N; ++i) x[i] = at + i < len ? (float)row[at + i] : fill;
+    }
+}
+
+// N fp32 values to the elements [at, at + N) of a row of `len`, rounded once; what lies behind the row's end is dropped.
+template <class T, int N> __device__ __forceinline__ void store_values(T* row, int64_t at, int64_t len, const float* x) {
+    if (at + N <= len) {
+        T v[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = (T)x[i];
+        __builtin_memcpy(row + at, v, N * sizeof(T));
+    } else {
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (at + i < len) row[at + i] = (T)x[i];
+    }
+}
+
+// host side: vdb_value_type codes to template arguments
+static inline bool valid_type(int type) { return type == VDB_VALUE_F32 || type == VDB_VALUE_BF16 || type == VDB_VALUE_F16; }
+
+template <class F> static int with_type(int type, F&& f) {
+    if (type == VDB_VALUE_F32) return f((float*)nullptr);
+    if (type == VDB_VALUE_BF16) return f((bf16_t*)nullptr);
+    return f((f16_t*)nullptr);
+}
+
+}  // namespace vdb

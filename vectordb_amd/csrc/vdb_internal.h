@@ -504,4 +504,8 @@ int launch_km_pp_step(const float* dist, int64_t n, bool first, float* nearest, 
 int launch_km_pp_select(const float* nearest, int64_t n, const double* block_sums, double u, long long* chosen,
                         long long* bad_weights, const KmNextQuery& nx, hipStream_t s);
 
+// out[i] = scale * table[rows[i]] (lookup.hip)
+int launch_lookup(const void* table, int table_type, int64_t n_rows, int dim, int64_t ld, const int64_t* rows, int64_t n, float scale,
+                  void* out, int out_type, int64_t ld_out, hipStream_t s);
+
 }  // namespace vdb
