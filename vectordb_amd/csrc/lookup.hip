@@ -56,8 +56,9 @@ static SortPlan sort_plan(int64_t n, int64_t n_rows) {
     while (((int64_t)1 << key_bits) <= n_rows) ++key_bits;
     p.passes = (key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     p.bits = (key_bits + p.passes - 1) / p.passes;
-    // 512 keys a wave until there are 1024 blocks, more beyond
-    p.wave_keys = std::max<int64_t>(512, round_up64((n + 1024 * SORT_WAVES - 1) / (1024 * SORT_WAVES), 64));
+    // a wave takes its keys 64 at a time, each step waiting for the last: few of them, until the blocks' histograms
+    // would outgrow what they save (512 blocks)
+    p.wave_keys = std::max<int64_t>(128, round_up64((n + 512 * SORT_WAVES - 1) / (512 * SORT_WAVES), 64));
     p.blocks = (int)((n + p.wave_keys * SORT_WAVES - 1) / (p.wave_keys * SORT_WAVES));
     return p;
 }
@@ -171,8 +172,104 @@ __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __
     }
 }
 
+// Up to SORT_ONE_MAX positions: the whole sort in one block, the pairs in LDS between the digits.
+static constexpr int SORT_ONE_NT = 1024, SORT_ONE_WAVES = SORT_ONE_NT / 64, SORT_ONE_ITEMS = 8, SORT_ONE_MAX = SORT_ONE_NT * SORT_ONE_ITEMS;
+
+__global__ void __launch_bounds__(SORT_ONE_NT) sort_one_kernel(const int64_t* __restrict__ rows, int n, int64_t n_rows, int bits, int passes,
+                                                               int* __restrict__ keys_out, int* __restrict__ pos_out) {
+    extern __shared__ int lds[];
+    const int bins = 1 << bits, room = (n + 63) & ~63;
+    int* skey = lds;
+    int* spos = lds + room;
+    int* start = lds + 2 * room;                       // [SORT_ONE_WAVES][bins]
+    __shared__ int wave_total[SORT_ONE_WAVES];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int per = ((n + SORT_ONE_WAVES - 1) / SORT_ONE_WAVES + 63) & ~63;
+    const int lo = min(wave * per, n), hi = min(lo + per, n);
+    int* mine = start + wave * bins;
+    int key[SORT_ONE_ITEMS], pos[SORT_ONE_ITEMS];
+    for (int pass = 0; pass < passes; ++pass) {
+        const int shift = pass * bits;
+        for (int d = tid; d < SORT_ONE_WAVES * bins; d += SORT_ONE_NT) start[d] = 0;
+#pragma unroll
+        for (int q = 0; q < SORT_ONE_ITEMS; ++q) {
+            const int i = lo + q * 64 + lane;
+            key[q] = 0;
+            pos[q] = i;
+            if (i < hi) {
+                key[q] = pass == 0 ? key_of(rows, nullptr, i, n_rows) : skey[i];
+                if (pass > 0) pos[q] = spos[i];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < SORT_ONE_ITEMS; ++q)
+            if (lo + q * 64 + lane < hi) atomicAdd(&mine[(key[q] >> shift) & (bins - 1)], 1);
+        __syncthreads();
+        // one digit a thread: prefix over the digits, then over the waves of a digit
+        int total = 0;
+        if (tid < bins)
+            for (int w = 0; w < SORT_ONE_WAVES; ++w) total += start[w * bins + tid];
+        int inc = total;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int t = __shfl_up(inc, o);
+            if (lane >= o) inc += t;
+        }
+        if (lane == 63) wave_total[wave] = inc;
+        __syncthreads();
+        int at = inc - total;
+        for (int w = 0; w < wave; ++w) at += wave_total[w];
+        if (tid < bins)
+            for (int w = 0; w < SORT_ONE_WAVES; ++w) {
+                const int c = start[w * bins + tid];
+                start[w * bins + tid] = at;
+                at += c;
+            }
+        __syncthreads();
+        const bool last = pass + 1 == passes;
+#pragma unroll
+        for (int q = 0; q < SORT_ONE_ITEMS; ++q) {
+            const int i0 = lo + q * 64;
+            if (i0 >= hi) break;
+            const bool have = i0 + lane < hi;
+            const int d = (key[q] >> shift) & (bins - 1);
+            const unsigned long long m = same_digit(d, bits, have);
+            if (have) {
+                const int rank = __popcll(m & ((1ull << lane) - 1));
+                const int base = mine[d];
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                if (rank == __popcll(m) - 1) mine[d] = base + rank + 1;
+                if (last) {
+                    keys_out[base + rank] = key[q];
+                    pos_out[base + rank] = pos[q];
+                } else {
+                    skey[base + rank] = key[q];
+                    spos[base + rank] = pos[q];
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        }
+        __syncthreads();
+    }
+}
+
 // ---------------------------------------------------------------- sums of the sorted rows
-static constexpr int SEG_CHUNK = 32;
+// Positions of a chunk: the rows of a batch of SEG_BATCH are in flight together.  Chunks of 32 where that fills the chip,
+// else of 8 (10240 rows of 384 values: 22 us with 32).
+static constexpr int SEG_BATCH = 8;
+
+// first position whose key is not below r, found by a whole wave: 64 probes a step (n and keys are below 2^31)
+__device__ __forceinline__ int64_t lower_bound_wave(const int* __restrict__ keys, int64_t n, int64_t r) {
+    uint32_t a = 0, b = (uint32_t)n;                       // the answer lies in [a, b]
+    while (a < b) {
+        const uint32_t step = (b - a + 63) >> 6, at = a + step * ((threadIdx.x & 63) + 1) - 1;
+        const uint32_t below = (uint32_t)__popcll(__ballot(at < b && (int64_t)keys[at < b ? at : a] < r));
+        b = min(b, a + step * (below + 1) - 1);
+        a += step * below;
+    }
+    return a;
+}
 
 template <class To, int N> __device__ __forceinline__ void put_row(To* row, int c, int dim, float scale, const float* acc, bool accumulate) {
     float x[N];
@@ -186,83 +283,155 @@ template <class To, int N> __device__ __forceinline__ void put_row(To* row, int 
     store_values<To, N>(row, c, dim, x);
 }
 
-// A group of 1 << log_tpr threads takes the chunk of SEG_CHUNK sorted positions g; columns in slices of blockIdx.y.
-// A row that neither starts before the chunk nor goes on behind it is finished here; the part of a row that started
-// before goes to part[g][0], of one that starts here and goes on to part[g][1].
+static constexpr int ZERO_ROWS = 64;
+
+// Blocks below zero_from: a group of 1 << log_tpr threads takes the chunk g of sorted positions; columns in slices of
+// blockIdx.y.  A row that neither starts before the chunk nor goes on behind it is finished here; the part of a row that
+// started before goes to part[g][0], of one that starts here and goes on to part[g][1].
+// The other blocks write zeros to those of ZERO_ROWS table rows that no position names (slice 0 alone).
 template <class Tg, class To>
 __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ grad, int64_t ld, const int* __restrict__ keys,
                                                       const int* __restrict__ pos, int64_t n, float scale, To* __restrict__ out,
                                                       int64_t n_rows, int dim, int64_t ld_out, int accumulate, float* __restrict__ part,
-                                                      int64_t chunks, int log_tpr) {
+                                                      int chunk, int64_t chunks, int log_tpr, int zero_from, int log_zero) {
+    if ((int)blockIdx.x >= zero_from) {
+        if (blockIdx.y) return;
+        __shared__ int64_t range[2];
+        __shared__ int named[ZERO_ROWS];
+        const int64_t r0 = (int64_t)((int)blockIdx.x - zero_from) * ZERO_ROWS;
+        if (threadIdx.x < ZERO_ROWS) named[threadIdx.x] = 0;
+        if (threadIdx.x < 128) {
+            const int64_t at = lower_bound_wave(keys, n, r0 + (threadIdx.x >> 6) * ZERO_ROWS);
+            if ((threadIdx.x & 63) == 0) range[threadIdx.x >> 6] = at;
+        }
+        __syncthreads();
+        for (int64_t p = range[0] + threadIdx.x; p < range[1]; p += 256) named[keys[p] - r0] = 1;
+        __syncthreads();
+        constexpr int N = Piece<To>::N;
+        float x[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) x[e] = 0.0f;
+        for (int j = threadIdx.x >> log_zero; j < ZERO_ROWS && r0 + j < n_rows; j += 256 >> log_zero) {
+            if (named[j]) continue;
+            To* dst = out + (r0 + j) * ld_out;
+            for (int c = (threadIdx.x & ((1 << log_zero) - 1)) * N; c < dim; c += N << log_zero) store_values<To, N>(dst, c, dim, x);
+        }
+        return;
+    }
     constexpr int N = Piece<Tg>::N;
     const int64_t g = (int64_t)blockIdx.x * (256 >> log_tpr) + (threadIdx.x >> log_tpr);
     const int c = ((blockIdx.y << log_tpr) + (threadIdx.x & ((1 << log_tpr) - 1))) * N;
     if (g >= chunks || c >= dim) return;
-    const int64_t p0 = g * SEG_CHUNK, p1 = min(p0 + SEG_CHUNK, n);
+    const int64_t p0 = g * chunk, p1 = min(p0 + chunk, n);
     const int before = p0 > 0 ? keys[p0 - 1] : -1, behind = p1 < n ? keys[p1] : -1;
+    const bool whole = c + N <= dim;
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0f;
-    int cur = keys[p0];
-    for (int64_t p = p0; p < p1 && cur < n_rows; ++p) {
-        float x[N];
-        load_values(grad + (int64_t)pos[p] * ld, c, dim, 0.0f, x);
+    for (int64_t b = p0; b < p1; b += SEG_BATCH) {
+        int key[SEG_BATCH + 1];
+        Piece<Tg> x[SEG_BATCH];
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += x[e];
-        const int next = p + 1 < p1 ? keys[p + 1] : -1;
-        if (next == cur) continue;
-        const bool open = p + 1 == p1 && behind == cur;
-        if (cur == before || open) store_values<float, N>(part + (g * 2 + (cur == before ? 0 : 1)) * dim, c, dim, acc);
-        else put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
+        for (int q = 0; q <= SEG_BATCH; ++q) key[q] = b + q < p1 ? keys[b + q] : -1;
 #pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] = 0.0f;
-        cur = next < 0 ? cur : next;
+        for (int q = 0; q < SEG_BATCH; ++q) {
+            if (key[q] < 0 || key[q] >= n_rows) continue;
+            const Tg* src = grad + (int64_t)pos[b + q] * ld;
+            if (whole) x[q] = load_piece(src + c);
+            else {
+                float v[N];
+                load_values(src, c, dim, 0.0f, v);
+                x[q].set(v);
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < SEG_BATCH; ++q) {
+            const int cur = key[q];
+            if (cur < 0 || cur >= n_rows) break;         // the positions without a row come last
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] += x[q].get(e);
+            if (key[q + 1] == cur) continue;
+            const bool open = b + q + 1 == p1 && behind == cur;
+            if (cur == before || open) store_values<float, N>(part + (g * 2 + (cur == before ? 0 : 1)) * dim, c, dim, acc);
+            else put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
+#pragma unroll
+            for (int e = 0; e < N; ++e) acc[e] = 0.0f;
+        }
     }
 }
 
-// The rows that cross chunks: the chunk in which such a row starts adds the parts of the following ones in order.
+// The rows that cross chunks.  A block looks at JOIN_CHUNKS chunks and takes 256 columns (blockIdx.y): a row that starts
+// in one of them and goes on has its parts, here and in the following chunks, added in order; up to SEG_BATCH parts by one
+// wave (the block's waves take such rows side by side), more by all waves, a contiguous run of parts each.  What takes the
+// time is the latency of the parts' loads (2 us a batch: other XCDs wrote them), so as many as possible are in flight.
+static constexpr int JOIN_NT = 1024, JOIN_WAVES = JOIN_NT / 64, JOIN_CHUNKS = 32;
+
+// parts [lo, hi) of the row that starts in chunk g: [g][1], then [g + 1][0], [g + 2][0], ...
+template <int N> __device__ __forceinline__ void add_parts(const float* part, int64_t g, int64_t lo, int64_t hi, int c, int dim, float* acc) {
+    for (int64_t j = lo; j < hi; j += SEG_BATCH) {
+        float x[SEG_BATCH][N];
+#pragma unroll
+        for (int q = 0; q < SEG_BATCH; ++q)
+            if (j + q < hi) load_values(part + ((g + j + q) * 2 + (j + q == 0 ? 1 : 0)) * dim, c, dim, 0.0f, x[q]);
+#pragma unroll
+        for (int q = 0; q < SEG_BATCH; ++q)
+            if (j + q < hi) {
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e] += x[q][e];
+            }
+    }
+}
+
 template <class To>
-__global__ void __launch_bounds__(256) seg_join_kernel(const int* __restrict__ keys, int64_t n, float scale, To* __restrict__ out, int64_t n_rows,
-                                                       int dim, int64_t ld_out, int accumulate, const float* __restrict__ part, int64_t chunks,
-                                                       int log_tpr) {
+__global__ void __launch_bounds__(JOIN_NT) seg_join_kernel(const int* __restrict__ keys, int64_t n, float scale, To* __restrict__ out, int64_t n_rows,
+                                                           int dim, int64_t ld_out, int accumulate, const float* __restrict__ part, int chunk,
+                                                           int64_t chunks) {
     constexpr int N = 4;
-    const int64_t g = (int64_t)blockIdx.x * (256 >> log_tpr) + (threadIdx.x >> log_tpr);
-    const int c = ((blockIdx.y << log_tpr) + (threadIdx.x & ((1 << log_tpr) - 1))) * N;
-    if (g + 1 >= chunks || c >= dim) return;
-    const int64_t p0 = g * SEG_CHUNK;
-    const int cur = keys[p0 + SEG_CHUNK - 1];
-    if (cur >= n_rows || keys[p0 + SEG_CHUNK] != cur || (p0 > 0 && keys[p0 - 1] == cur)) return;
-    float acc[N];
-    load_values(part + (g * 2 + 1) * dim, c, dim, 0.0f, acc);
-    for (int64_t h = g + 1; h < chunks; ++h) {
-        float x[N];
-        load_values(part + h * 2 * dim, c, dim, 0.0f, x);
-#pragma unroll
-        for (int e = 0; e < N; ++e) acc[e] += x[e];
-        const int64_t end = (h + 1) * SEG_CHUNK;
-        if (end >= n || keys[end] != cur) break;
+    __shared__ float sums[JOIN_WAVES][256];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c = blockIdx.y * 256 + lane * N;
+    const bool active = c < dim;
+    bool starts = false, many = false;
+    {
+        const int64_t g = (int64_t)blockIdx.x * JOIN_CHUNKS + lane, p1 = (g + 1) * chunk;
+        if (lane < JOIN_CHUNKS && g + 1 < chunks) {
+            const int cur = keys[p1 - 1];
+            starts = cur < n_rows && keys[p1] == cur && !(g > 0 && keys[p1 - chunk - 1] == cur);
+            const int64_t far = (g + SEG_BATCH) * chunk;            // the first position of part number SEG_BATCH
+            many = starts && far < n && keys[far] == cur;
+        }
     }
-    put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
-}
-
-// zeros for the rows that no position names
-template <class To>
-__global__ void __launch_bounds__(256) seg_zero_kernel(const int* __restrict__ keys, int64_t n, To* __restrict__ out, int64_t n_rows, int dim,
-                                                       int64_t ld_out, int log_tpr) {
-    constexpr int N = Piece<To>::N;
-    const int64_t r = (int64_t)blockIdx.x * (256 >> log_tpr) + (threadIdx.x >> log_tpr);
-    if (r >= n_rows) return;
-    int64_t lo = 0, hi = n;
-    while (lo < hi) {
-        const int64_t mid = (lo + hi) >> 1;
-        if (keys[mid] < r) lo = mid + 1;
-        else hi = mid;
+    const unsigned long long few = __ballot(starts && !many), long_ones = __ballot(many);
+    int turn = 0;
+    for (unsigned long long todo = few; todo; todo &= todo - 1, ++turn) {
+        if (turn % JOIN_WAVES != wave) continue;
+        const int64_t g = (int64_t)blockIdx.x * JOIN_CHUNKS + __builtin_ctzll(todo);
+        const int cur = keys[(g + 1) * chunk - 1];
+        int count = 1;
+        for (int64_t p = (g + 1) * chunk; count < SEG_BATCH && p < n && keys[p] == cur; p += chunk) ++count;
+        if (!active) continue;
+        float acc[N] = {0.0f, 0.0f, 0.0f, 0.0f};
+        add_parts<N>(part, g, 0, count, c, dim, acc);
+        put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
     }
-    if (lo < n && keys[lo] == r) return;
-    float x[N];
+    for (unsigned long long todo = long_ones; todo; todo &= todo - 1) {
+        const int64_t g = (int64_t)blockIdx.x * JOIN_CHUNKS + __builtin_ctzll(todo);
+        const int cur = keys[(g + 1) * chunk - 1];
+        const int64_t end = lower_bound_wave(keys, n, (int64_t)cur + 1), count = (end - 1) / chunk - g + 1;
+        const int64_t per = (count + JOIN_WAVES - 1) / JOIN_WAVES, lo = wave * per, hi = lo + per < count ? lo + per : count;
+        float acc[N] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (active) add_parts<N>(part, g, lo, hi, c, dim, acc);
+        __syncthreads();
 #pragma unroll
-    for (int e = 0; e < N; ++e) x[e] = 0.0f;
-    for (int c = (threadIdx.x & ((1 << log_tpr) - 1)) * N; c < dim; c += N << log_tpr) store_values<To, N>(out + r * ld_out, c, dim, x);
+        for (int e = 0; e < N; ++e) sums[wave][lane * N + e] = acc[e];
+        __syncthreads();
+        if (wave == 0 && active) {
+            for (int w = 1; w < JOIN_WAVES; ++w)
+#pragma unroll
+                for (int e = 0; e < N; ++e) acc[e] += sums[w][lane * N + e];
+            put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
+        }
+    }
 }
 
 // threads per row: a power of two that covers the row's pieces, at most a block
@@ -271,6 +440,7 @@ static int log_threads(int pieces) {
     while (l < 8 && (1 << l) < pieces) ++l;
     return l;
 }
+
 int launch_lookup(const void* table, int table_type, int64_t n_rows, int dim, int64_t ld, const int64_t* rows, int64_t n, float scale,
                   void* out, int out_type, int64_t ld_out, hipStream_t s) {
     if (n <= 0) return VDB_OK;
@@ -293,9 +463,13 @@ struct GradWork {
     float* part;
     int64_t bytes;
 };
+static int seg_chunk(int64_t n, int dim) {
+    if (n <= 32) return 32;                                           // a single chunk needs no second launch
+    return n * ((dim + 3) / 4) / 32 >= (int64_t)256 * 1024 ? 32 : 8;
+}
 static GradWork grad_work(void* base, int64_t n, int64_t n_rows, int dim) {
     const SortPlan p = sort_plan(n, n_rows);
-    GradWork w;
+    GradWork w{};
     char* at = (char*)base;
     auto take = [&](int64_t bytes) {
         char* here = at;
@@ -304,19 +478,31 @@ static GradWork grad_work(void* base, int64_t n, int64_t n_rows, int dim) {
     };
     for (int i = 0; i < 2; ++i) w.keys[i] = (int*)take(n * 4);
     for (int i = 0; i < 2; ++i) w.pos[i] = (int*)take(n * 4);
-    w.hist = (int*)take(((int64_t)p.blocks << p.bits) * 4);
-    w.totals = (int*)take(((int64_t)1 << p.bits) * 4);
-    w.part = (float*)take((n + SEG_CHUNK - 1) / SEG_CHUNK * 2 * dim * 4);
+    if (n > SORT_ONE_MAX) {
+        w.hist = (int*)take(((int64_t)p.blocks << p.bits) * 4);
+        w.totals = (int*)take(((int64_t)1 << p.bits) * 4);
+    }
+    const int chunk = seg_chunk(n, dim);
+    w.part = (float*)take((n + chunk - 1) / chunk * 2 * dim * 4);
     w.bytes = at - (char*)base;
     return w;
 }
 
-static int launch_lookup_grad(const void* grad, int grad_type, int64_t ld, const int64_t* rows, int64_t n, float scale, void* out, int out_type,
-                              int64_t n_rows, int dim, int64_t ld_out, int accumulate, void* work, hipStream_t s) {
-    const GradWork w = grad_work(work, n, n_rows, dim);
+static int launch_sort(const int64_t* rows, int64_t n, int64_t n_rows, const GradWork& w, const int** keys, const int** pos, hipStream_t s) {
     const SortPlan p = sort_plan(n, n_rows);
     const int bins = 1 << p.bits;
-    for (int pass = 0; pass < p.passes && n > 0; ++pass) {
+    *keys = w.keys[(p.passes + 1) & 1];
+    *pos = w.pos[(p.passes + 1) & 1];
+    if (n <= 0) return VDB_OK;
+    if (n <= SORT_ONE_MAX) {
+        const size_t lds = (2 * (size_t)round_up64(n, 64) + (size_t)SORT_ONE_WAVES * bins) * 4;
+        VDB_TRY(raise_dynamic_lds((const void*)sort_one_kernel, (2 * (size_t)SORT_ONE_MAX + ((size_t)SORT_ONE_WAVES << SORT_MAX_BITS)) * 4));
+        hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(SORT_ONE_NT), lds, s, rows, (int)n, n_rows, p.bits, p.passes, const_cast<int*>(*keys),
+                           const_cast<int*>(*pos));
+        VDB_HIP(hipGetLastError());
+        return VDB_OK;
+    }
+    for (int pass = 0; pass < p.passes; ++pass) {
         const int64_t* src_rows = pass == 0 ? rows : nullptr;
         const int* src_keys = pass == 0 ? nullptr : w.keys[(pass + 1) & 1];
         const int* src_pos = pass == 0 ? nullptr : w.pos[(pass + 1) & 1];
@@ -329,27 +515,31 @@ static int launch_lookup_grad(const void* grad, int grad_type, int64_t ld, const
                            n_rows, pass * p.bits, p.bits, p.wave_keys, w.hist, w.totals, w.keys[pass & 1], w.pos[pass & 1]);
         VDB_HIP(hipGetLastError());
     }
-    const int* keys = w.keys[(p.passes + 1) & 1];
-    const int* pos = w.pos[(p.passes + 1) & 1];
-    const int64_t chunks = (n + SEG_CHUNK - 1) / SEG_CHUNK;
+    return VDB_OK;
+}
+
+static int launch_lookup_grad(const void* grad, int grad_type, int64_t ld, const int64_t* rows, int64_t n, float scale, void* out, int out_type,
+                              int64_t n_rows, int dim, int64_t ld_out, int accumulate, void* work, hipStream_t s) {
+    const GradWork w = grad_work(work, n, n_rows, dim);
+    const int *keys = nullptr, *pos = nullptr;
+    VDB_TRY(launch_sort(rows, n, n_rows, w, &keys, &pos, s));
+    const int chunk = seg_chunk(n, dim);
+    const int64_t chunks = (n + chunk - 1) / chunk;
     return with_type(out_type, [&](auto* to) -> int {
         typedef std::remove_pointer_t<decltype(to)> To;
-        if (!accumulate) {
-            const int l = log_threads((dim + Piece<To>::N - 1) / Piece<To>::N);
-            hipLaunchKernelGGL((seg_zero_kernel<To>), dim3(ceil_div(n_rows, 256 >> l)), dim3(256), 0, s, keys, n, (To*)out, n_rows, dim, ld_out, l);
-            VDB_HIP(hipGetLastError());
-        }
-        if (n <= 0) return VDB_OK;
         return with_type(grad_type, [&](auto* tg) -> int {
             typedef std::remove_pointer_t<decltype(tg)> Tg;
             const int pieces = (dim + Piece<Tg>::N - 1) / Piece<Tg>::N, l = log_threads(pieces);
-            hipLaunchKernelGGL((seg_sum_kernel<Tg, To>), dim3(ceil_div(chunks, 256 >> l), ceil_div(pieces, 1 << l)), dim3(256), 0, s, (const Tg*)grad,
-                               ld, keys, pos, n, scale, (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunks, l);
+            const int lz = log_threads((dim + Piece<To>::N - 1) / Piece<To>::N);
+            const int sums = ceil_div(chunks, 256 >> l), zeros = accumulate ? 0 : ceil_div(n_rows, ZERO_ROWS);
+            hipLaunchKernelGGL((seg_sum_kernel<Tg, To>), dim3(sums + zeros, ceil_div(pieces, 1 << l)), dim3(256), 0, s, (const Tg*)grad, ld, keys, pos,
+                               n, scale, (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks, l, sums, lz);
             VDB_HIP(hipGetLastError());
-            const int joins = (dim + 3) / 4, lj = log_threads(joins);
-            hipLaunchKernelGGL((seg_join_kernel<To>), dim3(ceil_div(chunks, 256 >> lj), ceil_div(joins, 1 << lj)), dim3(256), 0, s, keys, n, scale,
-                               (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunks, lj);
-            VDB_HIP(hipGetLastError());
+            if (chunks > 1) {
+                hipLaunchKernelGGL((seg_join_kernel<To>), dim3(ceil_div(chunks - 1, JOIN_CHUNKS), ceil_div(dim, 256)), dim3(JOIN_NT), 0, s, keys, n, scale,
+                                   (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks);
+                VDB_HIP(hipGetLastError());
+            }
             return VDB_OK;
         });
     });
