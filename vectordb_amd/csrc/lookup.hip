@@ -69,17 +69,39 @@ __device__ __forceinline__ int key_of(const int64_t* rows, const int* keys, int6
     return (int)(r >= 0 && r < n_rows ? r : n_rows);
 }
 
+// Zeros for table rows, written by blocks behind those of a sort launch: the sort waits on latencies and leaves the
+// memory idle.  Rows [r0, r1) of `units` 16-bit units, `ld` units apart; a group of 1 << log_tpr threads takes a row.
+struct Fill {
+    uint16_t* out;
+    int64_t r0, r1, units, ld;
+    int log_tpr;
+};
+__device__ static void fill_rows(const Fill& f, int64_t block, int64_t blocks, int nt) {
+    const int per = nt >> f.log_tpr;
+    const u32x4 zero = {0u, 0u, 0u, 0u};
+    for (int64_t r = f.r0 + block * per + (threadIdx.x >> f.log_tpr); r < f.r1; r += blocks * per) {
+        uint16_t* dst = f.out + r * f.ld;
+        for (int64_t c = (threadIdx.x & ((1 << f.log_tpr) - 1)) * 8; c < f.units; c += (int64_t)8 << f.log_tpr) {
+            if (c + 8 <= f.units) __builtin_memcpy(dst + c, &zero, 16);
+            else
+                for (int64_t e = c; e < f.units; ++e) dst[e] = 0;
+        }
+    }
+}
+
 // hist[digit][block]
 __global__ void __launch_bounds__(SORT_NT) sort_hist_kernel(const int64_t* __restrict__ rows, const int* __restrict__ keys, int64_t n,
-                                                            int64_t n_rows, int shift, int bits, int64_t wave_keys, int* __restrict__ hist) {
+                                                            int64_t n_rows, int shift, int bits, int64_t wave_keys, int* __restrict__ hist,
+                                                            int blocks, Fill fill) {
     extern __shared__ int cnt[];
+    if ((int)blockIdx.x >= blocks) return fill_rows(fill, (int)blockIdx.x - blocks, (int)gridDim.x - blocks, SORT_NT);
     const int bins = 1 << bits;
     for (int d = threadIdx.x; d < bins; d += SORT_NT) cnt[d] = 0;
     __syncthreads();
     const int64_t lo = (int64_t)blockIdx.x * wave_keys * SORT_WAVES, hi = min(lo + wave_keys * SORT_WAVES, n);
     for (int64_t i = lo + threadIdx.x; i < hi; i += SORT_NT) atomicAdd(&cnt[(key_of(rows, keys, i, n_rows) >> shift) & (bins - 1)], 1);
     __syncthreads();
-    for (int d = threadIdx.x; d < bins; d += SORT_NT) hist[(int64_t)d * gridDim.x + blockIdx.x] = cnt[d];
+    for (int d = threadIdx.x; d < bins; d += SORT_NT) hist[(int64_t)d * blocks + blockIdx.x] = cnt[d];
 }
 
 // one wave per digit: exclusive prefix of its counts over the blocks, and their total
@@ -114,8 +136,9 @@ __device__ __forceinline__ unsigned long long same_digit(int d, int bits, bool h
 __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __restrict__ rows, const int* __restrict__ keys,
                                                                const int* __restrict__ pos, int64_t n, int64_t n_rows, int shift, int bits,
                                                                int64_t wave_keys, const int* __restrict__ hist, const int* __restrict__ totals,
-                                                               int* __restrict__ keys_out, int* __restrict__ pos_out) {
+                                                               int* __restrict__ keys_out, int* __restrict__ pos_out, int blocks, Fill fill) {
     extern __shared__ int lds[];
+    if ((int)blockIdx.x >= blocks) return fill_rows(fill, (int)blockIdx.x - blocks, (int)gridDim.x - blocks, SORT_NT);
     const int bins = 1 << bits;
     int* start = lds;                         // [SORT_WAVES][bins]
     int* scan = lds + SORT_WAVES * bins;      // [SORT_NT]
@@ -144,7 +167,7 @@ __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __
     for (int j = 0; j < per; ++j) {
         const int d = tid * per + j;
         if (d >= bins) break;
-        int at = run + hist[(int64_t)d * gridDim.x + blockIdx.x];
+        int at = run + hist[(int64_t)d * blocks + blockIdx.x];
         run += totals[d];
         for (int w = 0; w < SORT_WAVES; ++w) {
             const int c = start[w * bins + d];
@@ -176,8 +199,9 @@ __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __
 static constexpr int SORT_ONE_NT = 1024, SORT_ONE_WAVES = SORT_ONE_NT / 64, SORT_ONE_ITEMS = 8, SORT_ONE_MAX = SORT_ONE_NT * SORT_ONE_ITEMS;
 
 __global__ void __launch_bounds__(SORT_ONE_NT) sort_one_kernel(const int64_t* __restrict__ rows, int n, int64_t n_rows, int bits, int passes,
-                                                               int* __restrict__ keys_out, int* __restrict__ pos_out) {
+                                                               int* __restrict__ keys_out, int* __restrict__ pos_out, Fill fill) {
     extern __shared__ int lds[];
+    if (blockIdx.x > 0) return fill_rows(fill, (int)blockIdx.x - 1, (int)gridDim.x - 1, SORT_ONE_NT);
     const int bins = 1 << bits, room = (n + 63) & ~63;
     int* skey = lds;
     int* spos = lds + room;
@@ -465,8 +489,15 @@ struct GradWork {
 };
 static int seg_chunk(int64_t n, int dim) {
     if (n <= 32) return 32;                                           // a single chunk needs no second launch
-    return n * ((dim + 3) / 4) / 32 >= (int64_t)256 * 1024 ? 32 : 8;
+    const int64_t lanes = n * ((dim + 3) / 4);
+    // 131072 x 2048: parts written and joined cost 37 us with chunks of 32, 20 us with 64, the sums 348 and 352 us
+    for (int chunk = 64; chunk > 8; chunk >>= 1)
+        if (lanes / chunk >= (int64_t)256 * 1024) return chunk;
+    return 8;
 }
+// Whether the whole table is zeroed beside the sort, and the named rows written over it: where those are few (10240 x 384
+// into 100000 rows: 22 us of zeros behind 30 us of sorting), else the sums' launch writes zeros to the other rows alone.
+static bool fill_first(int64_t n, int64_t n_rows) { return n > 0 && n <= n_rows / 4; }
 static GradWork grad_work(void* base, int64_t n, int64_t n_rows, int dim) {
     const SortPlan p = sort_plan(n, n_rows);
     GradWork w{};
@@ -488,31 +519,42 @@ static GradWork grad_work(void* base, int64_t n, int64_t n_rows, int dim) {
     return w;
 }
 
-static int launch_sort(const int64_t* rows, int64_t n, int64_t n_rows, const GradWork& w, const int** keys, const int** pos, hipStream_t s) {
+static int launch_sort(const int64_t* rows, int64_t n, int64_t n_rows, const GradWork& w, Fill fill, const int** keys, const int** pos, hipStream_t s) {
     const SortPlan p = sort_plan(n, n_rows);
     const int bins = 1 << p.bits;
     *keys = w.keys[(p.passes + 1) & 1];
     *pos = w.pos[(p.passes + 1) & 1];
     if (n <= 0) return VDB_OK;
+    // blocks of 32 KB of zeros or more, at most eight a CU
+    auto fill_blocks = [&](int64_t lo, int64_t hi, int threads) {
+        fill.r0 = lo;
+        fill.r1 = hi;
+        return (int)std::min<int64_t>(((hi - lo) * fill.units * 2 + 32767) / 32768, (int64_t)ctx().num_cus * 2048 / threads);
+    };
+    const int64_t fill_end = fill.out ? n_rows : 0;
     if (n <= SORT_ONE_MAX) {
         const size_t lds = (2 * (size_t)round_up64(n, 64) + (size_t)SORT_ONE_WAVES * bins) * 4;
         VDB_TRY(raise_dynamic_lds((const void*)sort_one_kernel, (2 * (size_t)SORT_ONE_MAX + ((size_t)SORT_ONE_WAVES << SORT_MAX_BITS)) * 4));
-        hipLaunchKernelGGL(sort_one_kernel, dim3(1), dim3(SORT_ONE_NT), lds, s, rows, (int)n, n_rows, p.bits, p.passes, const_cast<int*>(*keys),
-                           const_cast<int*>(*pos));
+        const int extra = fill_blocks(0, fill_end, SORT_ONE_NT);
+        hipLaunchKernelGGL(sort_one_kernel, dim3(1 + extra), dim3(SORT_ONE_NT), lds, s, rows, (int)n, n_rows, p.bits, p.passes, const_cast<int*>(*keys),
+                           const_cast<int*>(*pos), fill);
         VDB_HIP(hipGetLastError());
         return VDB_OK;
     }
+    const int shares = 2 * p.passes;
     for (int pass = 0; pass < p.passes; ++pass) {
         const int64_t* src_rows = pass == 0 ? rows : nullptr;
         const int* src_keys = pass == 0 ? nullptr : w.keys[(pass + 1) & 1];
         const int* src_pos = pass == 0 ? nullptr : w.pos[(pass + 1) & 1];
-        hipLaunchKernelGGL(sort_hist_kernel, dim3(p.blocks), dim3(SORT_NT), bins * 4, s, src_rows, src_keys, n, n_rows, pass * p.bits, p.bits,
-                           p.wave_keys, w.hist);
+        int extra = fill_blocks(fill_end * (2 * pass) / shares, fill_end * (2 * pass + 1) / shares, SORT_NT);
+        hipLaunchKernelGGL(sort_hist_kernel, dim3(p.blocks + extra), dim3(SORT_NT), bins * 4, s, src_rows, src_keys, n, n_rows, pass * p.bits, p.bits,
+                           p.wave_keys, w.hist, p.blocks, fill);
         VDB_HIP(hipGetLastError());
         hipLaunchKernelGGL(sort_scan_kernel, dim3(bins), dim3(64), 0, s, w.hist, p.blocks, w.totals);
         VDB_HIP(hipGetLastError());
-        hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks), dim3(SORT_NT), (SORT_WAVES * bins + SORT_NT) * 4, s, src_rows, src_keys, src_pos, n,
-                           n_rows, pass * p.bits, p.bits, p.wave_keys, w.hist, w.totals, w.keys[pass & 1], w.pos[pass & 1]);
+        extra = fill_blocks(fill_end * (2 * pass + 1) / shares, fill_end * (2 * pass + 2) / shares, SORT_NT);
+        hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks + extra), dim3(SORT_NT), (SORT_WAVES * bins + SORT_NT) * 4, s, src_rows, src_keys, src_pos,
+                           n, n_rows, pass * p.bits, p.bits, p.wave_keys, w.hist, w.totals, w.keys[pass & 1], w.pos[pass & 1], p.blocks, fill);
         VDB_HIP(hipGetLastError());
     }
     return VDB_OK;
@@ -522,7 +564,10 @@ static int launch_lookup_grad(const void* grad, int grad_type, int64_t ld, const
                               int64_t n_rows, int dim, int64_t ld_out, int accumulate, void* work, hipStream_t s) {
     const GradWork w = grad_work(work, n, n_rows, dim);
     const int *keys = nullptr, *pos = nullptr;
-    VDB_TRY(launch_sort(rows, n, n_rows, w, &keys, &pos, s));
+    const bool filled = !accumulate && fill_first(n, n_rows);
+    const int half = out_type == VDB_VALUE_F32 ? 2 : 1;              // 16-bit units of a value
+    const Fill fill{filled ? (uint16_t*)out : nullptr, 0, 0, (int64_t)dim * half, ld_out * half, log_threads((dim * half + 7) / 8)};
+    VDB_TRY(launch_sort(rows, n, n_rows, w, fill, &keys, &pos, s));
     const int chunk = seg_chunk(n, dim);
     const int64_t chunks = (n + chunk - 1) / chunk;
     return with_type(out_type, [&](auto* to) -> int {
@@ -531,7 +576,7 @@ static int launch_lookup_grad(const void* grad, int grad_type, int64_t ld, const
             typedef std::remove_pointer_t<decltype(tg)> Tg;
             const int pieces = (dim + Piece<Tg>::N - 1) / Piece<Tg>::N, l = log_threads(pieces);
             const int lz = log_threads((dim + Piece<To>::N - 1) / Piece<To>::N);
-            const int sums = ceil_div(chunks, 256 >> l), zeros = accumulate ? 0 : ceil_div(n_rows, ZERO_ROWS);
+            const int sums = ceil_div(chunks, 256 >> l), zeros = accumulate || filled ? 0 : ceil_div(n_rows, ZERO_ROWS);
             hipLaunchKernelGGL((seg_sum_kernel<Tg, To>), dim3(sums + zeros, ceil_div(pieces, 1 << l)), dim3(256), 0, s, (const Tg*)grad, ld, keys, pos,
                                n, scale, (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks, l, sums, lz);
             VDB_HIP(hipGetLastError());
