@@ -2,10 +2,17 @@
 // uniform number given by the caller.
 //
 // What remains of a row after the filters is a prefix of the order (score descending, row number ascending): a
-// smallest score and how many of the rows that share it.  That score is found without sorting: a histogram of the
-// scores' ordered bit patterns, eight bits at a time, counts (top-k) or adds weights (top-p) until one pattern is
-// left.  Weights exp((z - max) / tau) are taken in double and added as 64-bit integers (multiples of 2^-s), so sums do
-// not depend on the order in which threads add, and the draw is the one of the definition.
+// smallest score and how many of the rows that share it.  It is found without sorting:
+//   - top-k, or min-p alone, leaves few rows: those at or above a bound (no fewer than k rows reach the k-th largest of
+//     the maxima of k groups or more) go to a list in LDS, in row order, and everything else happens there;
+//   - top-p alone takes a histogram of the weights over the distance from the best score, and then the scores of the one
+//     bin in which the border lies, narrowed by their ordered bit patterns.
+// Weights exp((z - max) / tau) are taken in double, to 2^-50, and added as 64-bit integers (multiples of 2^-s): sums do not
+// depend on the order in which threads add, and the draw is the one of the definition.
+//
+// Two forms.  Short rows: a block of 1024 threads takes a row through all its passes.  Long rows are streamed by the whole
+// chip: one pass takes the maxima of groups of 32 scores (the floor: n * vocab values read once), a block per row finishes
+// the rows that a list settles from those maxima, and for the others two more passes add up weights.
 #include "vdb_internal.h"
 #include "values.h"
 
@@ -14,7 +21,9 @@
 namespace vdb {
 
 static constexpr int SAMPLE_NT = 1024, SAMPLE_WAVES = SAMPLE_NT / 64;
+static constexpr int LIST_MAX = 2048, LIST_ITEMS = LIST_MAX / SAMPLE_NT, BINS = 2 * SAMPLE_NT, EXP_STEPS = 1024, GROUPS = 64, AHEAD = 4;
 typedef unsigned long long u64;
+static constexpr float LOWEST = -3.4028234663852886e38f;
 
 struct SampleArgs {
     int64_t vocab, ld;
@@ -28,295 +37,669 @@ struct SampleArgs {
     int64_t* out_row; float* out_logp;
     int shift;                       // weights are multiples of 2^-shift
 };
+// what a row asks for
+struct Settings {
+    float tau, top_p, min_p, uniform;
+    int top_k;
+    __device__ __forceinline__ Settings(const SampleArgs& a, int64_t row)
+        : tau(a.d_temperature ? a.d_temperature[row] : a.temperature), top_p(a.d_top_p ? a.d_top_p[row] : a.top_p),
+          min_p(a.d_min_p ? a.d_min_p[row] : a.min_p), uniform(a.uniform[row]), top_k(a.d_top_k ? a.d_top_k[row] : a.top_k) {}
+    __device__ __forceinline__ bool first_of_best() const { return !(tau > 0.0f) || top_k == 1 || top_p <= 0.0f; }
+    __device__ __forceinline__ bool by_count() const { return top_k > 1; }
+    __device__ __forceinline__ bool by_mass() const { return top_p < 1.0f; }
+    __device__ __forceinline__ u64 least_weight(int shift) const {
+        return min_p > 0.0f ? (u64)ceil(fmin((double)min_p, 1.0) * (double)((u64)1 << shift)) : 0;
+    }
+    // no score below weighs min_p of the best
+    __device__ __forceinline__ float min_p_bound(float best) const {
+        const double lowest = (double)best + log(fmin((double)min_p, 1.0)) * (double)tau;
+        return (float)fmax(lowest - (fabs(lowest) + fabs((double)best)) * 1e-6, (double)LOWEST);
+    }
+    // running sum > uniform * total, as integers
+    __device__ __forceinline__ u64 goal(u64 total) const {
+        const double g = (double)uniform * (double)total;
+        const u64 least = g >= 0.0 ? (u64)floor(g) + 1 : 1;
+        return least <= total ? least : total;
+    }
+};
 
-// Ordered pattern of a score: larger score, larger pattern; 0 = cannot be drawn.  -0 counts as +0.
+// Ordered pattern of a score that can be drawn: larger score, larger pattern.  -0 counts as +0; 0 for NaN and -inf.
 __device__ __forceinline__ uint32_t pattern(float z) {
     const uint32_t b = __float_as_uint(z + 0.0f);
     const uint32_t o = (b & 0x80000000u) ? ~b : (b | 0x80000000u);
-    return (z != z || z == -INFINITY) ? 0u : o;
+    return z > -INFINITY ? o : 0u;
 }
 __device__ __forceinline__ float score_of(uint32_t o) { return __uint_as_float((o & 0x80000000u) ? (o & 0x7fffffffu) : ~o); }
 
-template <class T> struct Row {
+// A row's pieces: what cannot be drawn (filtered, behind the end) is -inf; a NaN fails every comparison and never counts.
+template <class T> struct Source {
     const T* z;
-    int64_t vocab;
+    int vocab;
     const uint32_t* mask;
-    int flip;
-    // ordered patterns of the elements [at, at + N)
-    __device__ __forceinline__ void load(int64_t at, uint32_t* o) const {
+    bool flip, infinite;             // infinite: the best is +inf; those rows weigh 1, the others nothing
+    static __device__ __forceinline__ uint32_t nothing() { return sizeof(T) == 4 ? 0xff800000u : (__is_same(T, bf16_t) ? 0xff80ff80u : 0xfc00fc00u); }
+    __device__ __forceinline__ Piece<T> load(int at) const {
         constexpr int N = Piece<T>::N;
-        float x[N];
-        load_values(z, at, vocab, NAN, x);
-        uint32_t bits = 0xffffffffu;
-        if (mask && at < vocab) bits = mask[at >> 5] >> (at & 31);      // N divides 32: one word holds the piece
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const uint32_t p = pattern(flip ? -x[e] : x[e]);
-            o[e] = (bits >> e) & 1u ? p : 0u;
+        Piece<T> x;
+        if (at + N <= vocab) x = load_piece(z + at);
+        else {
+            float v[N];
+            load_values(z, at, vocab, flip ? INFINITY : -INFINITY, v);
+            x.set(v);
         }
+        return x;
     }
-};
-
-struct Weigher {
-    double per_log2;                 // log2(e) / tau
-    uint32_t best;
-    double best_z, unit;
-    __device__ __forceinline__ u64 operator()(uint32_t o) const {
-        if (o == best) return (u64)unit;
-        const double t = ((double)score_of(o) - best_z) * per_log2;
-        return t >= -40.0 ? (u64)(exp2(t) * unit + 0.5) : 0ull;       // a NaN (tau = inf under scores of inf) is no weight
+    __device__ __forceinline__ Source(const T* scores, const SampleArgs& a, int64_t row)
+        : z(scores + row * a.ld), vocab((int)a.vocab), mask(a.mask ? a.mask + row * a.mask_ld : nullptr), flip(a.smaller_first != 0), infinite(false) {}
+    // one score
+    __device__ __forceinline__ float one(int at) const {
+        if (at >= vocab || (mask && !((mask[at >> 5] >> (at & 31)) & 1u))) return -INFINITY;
+        float x = (float)z[at];
+        if (flip) x = -x;
+        if (infinite) x = x == INFINITY ? 0.0f : -INFINITY;
+        return x > -INFINITY ? x : -INFINITY;
     }
-    __device__ __forceinline__ double exact(uint32_t o) const {
-        if (o == best) return 1.0;
-        return exp2(((double)score_of(o) - best_z) * per_log2);
-    }
-};
-
-__device__ __forceinline__ u64 wave_sum(u64 v) {
+    __device__ __forceinline__ uint32_t bits(int at) const { return mask && at < vocab ? mask[at >> 5] >> (at & 31) : 0xffffffffu; }   // N divides 32
+    __device__ __forceinline__ void finish(Piece<T>& x, uint32_t bits) const {
+        if (flip) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+            for (int i = 0; i < 4; ++i) x.raw[i] ^= sizeof(T) == 4 ? 0x80000000u : 0x80008000u;
+        }
+        if (mask) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                uint32_t keep;
+                if constexpr (sizeof(T) == 4) keep = 0u - ((bits >> i) & 1u);
+                else keep = ((0u - ((bits >> (2 * i)) & 1u)) & 0xffffu) | ((0u - ((bits >> (2 * i + 1)) & 1u)) << 16);
+                x.raw[i] = (x.raw[i] & keep) | (nothing() & ~keep);
+            }
+        }
+        if (infinite) only_infinite(x);
+    }
+    static __device__ __forceinline__ void only_infinite(Piece<T>& x) {
+        constexpr int N = Piece<T>::N;
+        float y[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) y[e] = x.get(e) == INFINITY ? 0.0f : -INFINITY;
+        x.set(y);
+    }
+};
+
+// The weight exp((z - best) / tau) as a multiple of 2^-s: with x = (z - best) c, c = 1024 log2(e) / tau, and k = x rounded,
+// 2^(x / 1024) = 2^(k >> 10) table[k & 1023] q(x - k), q a cubic (its remainder is below 2^-50 for |x - k| <= 1/2).  Adding
+// 2^(52 - s) leaves the multiple in the low mantissa bits.  About 18 instructions a score; exp2() of the library takes 40.
+struct FixedExp {
+    double best, c, round_to;        // round_to = 2^(52 - s)
+    float cut;                       // scores below weigh nothing (2^-40 of the best)
+    const double* table;             // 2^(j / 1024), in LDS
+    static constexpr double NEAREST = 6755399441055744.0;            // 1.5 * 2^52: the nearest integer in the low bits
+    __device__ __forceinline__ FixedExp(float best_, float tau, int shift, const double* t)
+        : best(best_), c(EXP_STEPS * 1.4426950408889634073599 / (double)tau), round_to((double)((u64)1 << (52 - shift))),
+          cut((float)fmax((double)best_ - 40.0 * 0.69314718055994530942 * (double)tau, (double)LOWEST)), table(t) {}
+    // scores of bin b lie in [*lo, *hi]; what else does is told apart by its bin
+    __device__ __forceinline__ void bin_range(int b, float* lo, float* hi) const {
+        const double h = best - (32.0 * b - 0.6) / c, l = best - (32.0 * b + 31.6) / c;
+        *hi = (float)fmin(best, h + fabs(h) * 2.4e-7);
+        *lo = (float)fmax(l - fabs(l) * 2.4e-7, (double)cut);
+    }
+    __device__ __forceinline__ int bin(float z) const {              // distance from the best in steps of 1/32 of a power of two
+        const int k = (int)(uint32_t)__double_as_longlong(fma((double)z - best, c, NEAREST));
+        return min((-k) >> 5, BINS - 1);
+    }
+    __device__ __forceinline__ u64 operator()(float z) const {
+        constexpr double L = 0.69314718055994530942 / EXP_STEPS;
+        const double d = (double)z - best;
+        const double a = fma(d, c, NEAREST);
+        const int k = (int)(uint32_t)__double_as_longlong(a);
+        const double f = fma(d, c, -(a - NEAREST));
+        double q = fma(f, L * L * L / 6, L * L / 2);
+        q = fma(f, q, L);
+        q = fma(f, q, 1.0);
+        const u64 t = (u64)__double_as_longlong(table[k & (EXP_STEPS - 1)]);
+        const double scale = __longlong_as_double((long long)(t + ((u64)(uint32_t)(k >> 10) << 52)));
+        const u64 r = (u64)__double_as_longlong(fma(scale, q, round_to)) - (u64)__double_as_longlong(round_to);
+        return z >= cut ? r : 0;
+    }
+};
+
+struct SampleShared {
+    double table[EXP_STEPS];
+    u64 bin[BINS];
+    float list_z[LIST_MAX];
+    uint32_t list_at[LIST_MAX];
+    u64 part[SAMPLE_WAVES * GROUPS];     // per part of the row, in row order: counts or weights, then their exclusive prefix
+    u64 before[256];
+    uint32_t rank[256];
+    u64 red[SAMPLE_WAVES];
+    u64 found_sum;
+    uint32_t found, first;
+};
+
+// Sums over a wave by data-parallel moves (rows of 16 lanes, then their last lanes passed on): a shuffle through LDS costs
+// a hundred cycles a step, and these stand once in every step of every pass.
+template <int CTRL, int ROWS> __device__ __forceinline__ u64 add_moved(u64 v) {
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), CTRL, ROWS, 0xf, false);
+    return v + (((u64)hi << 32) | lo);
+}
+__device__ __forceinline__ u64 wave_scan(u64 v) {
+    v = add_moved<0x111, 0xf>(v);        // row_shr:1, 2, 4, 8
+    v = add_moved<0x112, 0xf>(v);
+    v = add_moved<0x114, 0xf>(v);
+    v = add_moved<0x118, 0xf>(v);
+    v = add_moved<0x142, 0xa>(v);        // row_bcast:15 into rows 1 and 3
+    return add_moved<0x143, 0xc>(v);     // row_bcast:31 into rows 2 and 3
+}
+__device__ __forceinline__ u64 last_lane(u64 v) {
+    return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
+}
+__device__ __forceinline__ u64 wave_sum(u64 v) { return last_lane(wave_scan(v)); }
+// exclusive prefix of v over the block; *total = its sum
+__device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const u64 inc = wave_scan(v);
+    __syncthreads();
+    if (lane == 63) sh.red[wave] = inc;
+    __syncthreads();
+    u64 all = 0, base = 0;
+    for (int w = 0; w < SAMPLE_WAVES; ++w) {
+        if (w < wave) base += sh.red[w];
+        all += sh.red[w];
+    }
+    *total = all;
+    return base + inc - v;
+}
+__device__ __forceinline__ u64 block_total(SampleShared& sh, u64 v) {
+    v = wave_sum(v);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0;
+    for (int w = 0; w < SAMPLE_WAVES; ++w) v += sh.red[w];
     return v;
 }
-
-template <class T>
-__global__ void __launch_bounds__(SAMPLE_NT) sample_kernel(const T* __restrict__ scores, SampleArgs a) {
-    constexpr int N = Piece<T>::N;
-    __shared__ u64 bin[256];
-    __shared__ u64 red[SAMPLE_WAVES + 1];
-    __shared__ u64 chosen_above;
-    __shared__ int chosen_bin;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t row = blockIdx.x, vocab = a.vocab;
-    const Row<T> r{scores + row * a.ld, vocab, a.mask ? a.mask + row * a.mask_ld : nullptr, a.smaller_first};
-    const float tau = a.d_temperature ? a.d_temperature[row] : a.temperature;
-    const float top_p = a.d_top_p ? a.d_top_p[row] : a.top_p;
-    const float min_p = a.d_min_p ? a.d_min_p[row] : a.min_p;
-    const bool greedy = !(tau > 0.0f);
-    int64_t top_k = a.d_top_k ? a.d_top_k[row] : a.top_k;
-    if (greedy) top_k = 1;
-    const int64_t seg = (vocab + SAMPLE_WAVES - 1) / SAMPLE_WAVES;
-    const int64_t step = 64 * N, seg_len = (seg + step - 1) / step * step;          // a wave's contiguous part
-    const int64_t w_lo = min((int64_t)wave * seg_len, vocab), w_hi = min(w_lo + seg_len, vocab);
-
-    // the largest score
-    uint32_t best = 0;
-    for (int64_t i = (int64_t)tid * N; i < vocab; i += SAMPLE_NT * N) {
-        uint32_t o[N];
-        r.load(i, o);
-#pragma unroll
-        for (int e = 0; e < N; ++e) best = max(best, o[e]);
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) best = max(best, (uint32_t)__shfl_xor((int)best, o));
-    if (lane == 0) red[wave] = best;
+// the parts' exclusive prefix in place; -> their sum
+__device__ __forceinline__ u64 scan_parts(SampleShared& sh, int parts) {
     __syncthreads();
-    for (int w = 0; w < SAMPLE_WAVES; ++w) best = max(best, (uint32_t)red[w]);
-    if (best == 0) {
-        if (tid == 0) {
-            a.out_row[row] = -1;
-            if (a.out_logp) a.out_logp[row] = -INFINITY;
-        }
-        return;
+    const int tid = threadIdx.x;
+    u64 total;
+    const u64 v = block_scan(sh, tid < parts ? sh.part[tid] : 0, &total);
+    if (tid < parts) sh.part[tid] = v;
+    __syncthreads();
+    return total;
+}
+__device__ __forceinline__ void clear_bins(SampleShared& sh) {
+    __syncthreads();
+    sh.bin[threadIdx.x] = 0;
+    sh.bin[threadIdx.x + SAMPLE_NT] = 0;
+    __syncthreads();
+}
+__device__ __forceinline__ void make_table(double* table, int tid, int nt) {
+    for (int j = tid; j < EXP_STEPS; j += nt) table[j] = exp2((double)j / EXP_STEPS);
+}
+// the first bin, from the top or from the bottom, at which the running sum, from `above`, reaches target: sh.found its
+// number in that order (BINS: none), sh.found_sum the sum before it
+__device__ static void find_bin(SampleShared& sh, u64 above, u64 target, bool from_top) {
+    __syncthreads();
+    const int at = 2 * threadIdx.x;
+    const u64 v0 = sh.bin[from_top ? BINS - 1 - at : at], v1 = sh.bin[from_top ? BINS - 2 - at : at + 1];
+    u64 total;
+    if (threadIdx.x == 0) sh.found = BINS;
+    u64 run = above + block_scan(sh, v0 + v1, &total);          // its barriers order the write above with those below
+    if (run < target && run + v0 + v1 >= target) {
+        const bool second = run + v0 < target;
+        sh.found = (uint32_t)(at + (second ? 1 : 0));
+        sh.found_sum = run + (second ? v0 : 0);
     }
-    const Weigher weigh{1.4426950408889634073599 / (greedy ? 1.0 : (double)tau), best, (double)score_of(best), ldexp(1.0, a.shift)};
+    __syncthreads();
+}
 
-    // the prefix: scores above `cut`, and the first `ties` rows at it
-    uint32_t cut = 0;
-    int64_t ties = INT64_MAX;
-    // narrow to one pattern: the first, from the top, at which the running sum of `value` reaches `target`
-    auto narrow = [&](auto&& value, u64 target, u64* above_out) {
-        uint32_t known = 0;
-        u64 above = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) bin[tid] = 0;
-            __syncthreads();
-            for (int64_t i = (int64_t)tid * N; i < vocab; i += SAMPLE_NT * N) {
-                uint32_t o[N];
-                r.load(i, o);
+// The key, among those of each(f) in [lo, hi], at which the running sum of the weights, from the top and from `above`, reaches
+// target (0 < target; where it is not reached: lo); *sum_above = the sum before it.  each calls f(key, weight), weight a
+// function.  11 bits a step; after fewer steps than the range has bits, the smallest key that can still be it.
+template <class Each>
+__device__ __forceinline__ uint32_t narrow(SampleShared& sh, Each&& each, uint32_t lo, uint32_t hi, u64 above, u64 target, u64* sum_above, int steps = 3) {
+    for (; steps > 0 && lo < hi; --steps) {
+        const int shift = max(21 - __clz(hi - lo), 0);
+        clear_bins(sh);
+        each([&](uint32_t key, auto&& weight) {
+            if (key < lo || key > hi) return;
+            const u64 v = weight();
+            if (v) atomicAdd(&sh.bin[(key - lo) >> shift], v);
+        });
+        find_bin(sh, above, target, true);
+        const uint32_t found = sh.found;
+        if (found == BINS) break;
+        const uint32_t b = BINS - 1 - found;
+        above = sh.found_sum;
+        const uint32_t last = lo + ((b + 1) << shift) - 1;
+        if (last < hi) hi = last;
+        lo += b << shift;
+    }
+    *sum_above = above;
+    return lo;
+}
+__device__ __forceinline__ u64 one_each() { return 1; }
+
+__device__ __forceinline__ void write_draw(const SampleArgs& a, int64_t row, uint32_t at, u64 w, u64 total) {
+    a.out_row[row] = at;
+    if (a.out_logp) a.out_logp[row] = (float)log((double)w / (double)total);
+}
+__device__ __forceinline__ void write_certain(const SampleArgs& a, int64_t row, int64_t at) {
+    a.out_row[row] = at;
+    if (a.out_logp) a.out_logp[row] = at < 0 ? -INFINITY : 0.0f;
+}
+// how many rows at a cut remain whose weights before it are `above`: those with less than target before them
+__device__ __forceinline__ int64_t ties_within(double target, u64 above, u64 w) {
+    return max((int64_t)1, (int64_t)ceil((target - (double)above) / (double)w));
+}
+
+// ---------------------------------------------------------------- the draw from a list
+// `listed` <= LIST_MAX scores and their rows in sh.list_*, in row order, among them all that remain.
+__device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& a, int64_t row, const Settings& set, const FixedExp& weigh, int listed) {
+    const int tid = threadIdx.x;
+    const u64 least_w = set.least_weight(a.shift);
+    u64 w[LIST_ITEMS];
 #pragma unroll
-                for (int e = 0; e < N; ++e)
-                    if (o[e] && (shift == 24 || (o[e] >> (shift + 8)) == known)) {
-                        const u64 v = value(o[e]);
-                        if (v) atomicAdd(&bin[(o[e] >> shift) & 255], v);
-                    }
-            }
-            __syncthreads();
-            if (tid == 0) {
-                u64 run = above;
-                int b = 255;
-                for (; b > 0; --b) {
-                    if (run + bin[b] >= target) break;
-                    run += bin[b];
+    for (int q = 0; q < LIST_ITEMS; ++q) w[q] = q * SAMPLE_NT + tid < listed ? weigh(sh.list_z[q * SAMPLE_NT + tid]) : 0;
+    if (listed <= 256) {
+        // every item's rank and the weights before it, by comparing all pairs
+        int log_width = 6;
+        while ((1 << log_width) < listed) ++log_width;
+        const int i = tid & ((1 << log_width) - 1);
+        if (tid < 256) { sh.rank[tid] = 0; sh.before[tid] = 0; }
+        __syncthreads();
+        if (i < listed) {
+            const float zi = sh.list_z[i];
+            uint32_t rank = 0;
+            u64 before = 0;
+            for (int j = tid >> log_width; j < listed; j += SAMPLE_NT >> log_width) {
+                const float zj = sh.list_z[j];
+                if (zj > zi || (zj == zi && j < i)) {
+                    ++rank;
+                    if (set.by_mass()) before += weigh(zj);
                 }
-                chosen_above = run;
-                chosen_bin = b;
             }
-            __syncthreads();
-            above = chosen_above;
-            known = (known << 8) | (uint32_t)chosen_bin;
+            if (rank) {
+                atomicAdd(&sh.rank[i], rank);
+                if (set.by_mass()) atomicAdd(&sh.before[i], before);
+            }
         }
-        *above_out = above;
-        return known;
-    };
-    auto block_total = [&](u64 v) {
-        v = wave_sum(v);
         __syncthreads();
-        if (lane == 0) red[wave] = v;
-        __syncthreads();
-        v = 0;
-        for (int w = 0; w < SAMPLE_WAVES; ++w) v += red[w];
-        return v;
-    };
-    auto sum_over = [&](auto&& value) {
-        u64 v = 0;
-        for (int64_t i = (int64_t)tid * N; i < vocab; i += SAMPLE_NT * N) {
-            uint32_t o[N];
-            r.load(i, o);
-#pragma unroll
-            for (int e = 0; e < N; ++e)
-                if (o[e]) v += value(o[e]);
+        if (set.by_count() && tid < listed && sh.rank[tid] >= (uint32_t)set.top_k) w[0] = 0;
+        if (set.by_mass()) {
+            const double target = (double)block_total(sh, w[0]) * (double)set.top_p;
+            if (tid < listed && sh.rank[tid] > 0 && !((double)sh.before[tid] < target)) w[0] = 0;
         }
-        return block_total(v);
-    };
-
-    if (top_k > 0) {
-        const u64 usable = sum_over([](uint32_t) { return (u64)1; });
-        if ((u64)top_k < usable) {
+    } else {
+        float cut = -INFINITY;
+        int64_t ties = INT64_MAX;
+        const uint32_t top = pattern((float)weigh.best);
+        if (set.by_count() && set.top_k < listed) {
             u64 above;
-            cut = narrow([](uint32_t) { return (u64)1; }, (u64)top_k, &above);
-            ties = top_k - (int64_t)above;
+            cut = score_of(narrow(sh, [&](auto&& f) {
+                for (int i = tid; i < listed; i += SAMPLE_NT) f(pattern(sh.list_z[i]), one_each);
+            }, 1u, top, 0, (u64)set.top_k, &above));
+            ties = set.top_k - (int64_t)above;
+        }
+        if (set.by_mass()) {
+            u64 sum = 0;
+#pragma unroll
+            for (int q = 0; q < LIST_ITEMS; ++q)
+                if (w[q] && sh.list_z[q * SAMPLE_NT + tid] > cut) sum += w[q];
+            const u64 over = block_total(sh, sum), w_cut = ties < INT64_MAX ? weigh(cut) : 0;
+            const double target = (double)(over + w_cut * (u64)(ties < INT64_MAX ? ties : 0)) * (double)set.top_p;
+            const u64 least = max((u64)ceil(target), (u64)1);
+            if (over >= least) {
+                u64 above;
+                const float floor_z = cut;
+                cut = score_of(narrow(sh, [&](auto&& f) {
+                    for (int i = tid; i < listed; i += SAMPLE_NT) {
+                        const float z = sh.list_z[i];
+                        if (z > floor_z) f(pattern(z), [&] { return weigh(z); });
+                    }
+                }, 1u, top, 0, least, &above));
+                ties = ties_within(target, above, weigh(cut));
+            } else if (w_cut) {
+                ties = min(ties, ties_within(target, over, w_cut));
+            }
+        }
+        u64 run = 0;
+#pragma unroll
+        for (int q = 0; q < LIST_ITEMS; ++q) {
+            const int i = q * SAMPLE_NT + tid;
+            const bool at_cut = i < listed && sh.list_z[i] == cut;
+            u64 total;
+            const u64 before = run + block_scan(sh, at_cut ? 1 : 0, &total);
+            run += total;
+            if (i >= listed || sh.list_z[i] < cut || (at_cut && (int64_t)before >= ties)) w[q] = 0;
         }
     }
-    if (top_p < 1.0f) {
-        const u64 over = sum_over([&](uint32_t o) { return o > cut ? weigh(o) : 0ull; });
-        const u64 at_cut = cut && ties < INT64_MAX ? weigh(cut) * (u64)ties : 0ull;
-        const double target = (double)(over + at_cut) * (double)top_p;
-        // a row remains iff the weights before it are less than target: the first row is kept, and the last kept one is
-        // where the running sum, itself included, reaches the target
-        u64 least = target > 0.0 ? (u64)ceil(target) : 0ull;
-        if (least == 0) least = 1;
-        u64 above;
-        const uint32_t c2 = over && (double)over >= target ? narrow([&](uint32_t o) { return o > cut ? weigh(o) : 0ull; }, least, &above) : cut;
-        if (c2 != cut) {
-            const u64 w = weigh(c2);
-            const double left = (target - (double)above) / (double)w;
-            cut = c2;
-            ties = left >= 9.0e18 ? INT64_MAX : max((int64_t)1, (int64_t)ceil(left));
-        } else if (at_cut) {
-            const double left = (target - (double)over) / (double)weigh(cut);
-            ties = min(ties, max((int64_t)1, (int64_t)ceil(left)));
-        }
+    u64 before[LIST_ITEMS], all = 0;
+#pragma unroll
+    for (int q = 0; q < LIST_ITEMS; ++q) {
+        if (w[q] < least_w) w[q] = 0;
+        before[q] = 0;
+        if (q * SAMPLE_NT >= listed) continue;
+        u64 total;
+        before[q] = all + block_scan(sh, w[q], &total);
+        all += total;
     }
-    const double least_w = min_p > 0.0f ? fmin((double)min_p, 1.0) : 0.0;
-    const bool use_min = min_p > 0.0f;
-    if (use_min && cut && weigh.exact(cut) < least_w) ties = 0;
+    const u64 least = set.goal(all);
+#pragma unroll
+    for (int q = 0; q < LIST_ITEMS; ++q)
+        if (w[q] && before[q] < least && before[q] + w[q] >= least) write_draw(a, row, sh.list_at[q * SAMPLE_NT + tid], w[q], all);
+}
 
-    // the weight of a row at the cut counts for the first `ties` rows there, in row order
-    int64_t tie_end = vocab;                  // rows at the cut from here on are out
-    if (cut && ties < INT64_MAX) {
-        u64 mine = 0;
-        for (int64_t i = w_lo + lane * N; i < w_hi; i += step) {
-            uint32_t o[N];
-            r.load(i, o);
+// ---------------------------------------------------------------- a row by one block
+template <class T> struct RowPasses {
+    static constexpr int N = Piece<T>::N;
+    Source<T> src;
+    int tid, lane, wave;
+    // the parts of the row: a wave's contiguous share in up to GROUPS groups of `per_group` steps of 64 pieces
+    int steps, per_group, groups, parts, share;
+    __device__ __forceinline__ RowPasses(const Source<T>& s)
+        : src(s), tid(threadIdx.x), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
+        steps = ((src.vocab + SAMPLE_WAVES - 1) / SAMPLE_WAVES + 64 * N - 1) / (64 * N);
+        per_group = (steps + GROUPS - 1) / GROUPS;
+        groups = (steps + per_group - 1) / per_group;
+        parts = SAMPLE_WAVES * groups;
+        share = steps * 64 * N;
+    }
+    // Pieces of a loop, AHEAD loads in flight while the ones before are worked on: f(step, first element, piece) for steps
+    // [from, to), `at(step)` the first element of this lane's piece.  A step is kept apart from the next (sched_barrier): the
+    // compiler would interleave them and run out of registers.
+    template <class At, class F> __device__ __forceinline__ void pieces(int from, int to, At&& at, F&& f) const {
+        Piece<T> next[AHEAD];
+        uint32_t bits[AHEAD];
+        auto fetch = [&](int t0) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) mine += (i + e < w_hi && o[e] == cut) ? 1 : 0;
-        }
-        mine = wave_sum(mine);
-        __syncthreads();
-        if (lane == 0) red[wave] = mine;
-        if (tid == 0) chosen_above = (u64)vocab;
-        __syncthreads();
-        int64_t run = 0;
-        for (int w = 0; w < wave; ++w) run += (int64_t)red[w];
-        if (run <= ties && run + (int64_t)mine > ties) {
-            // the first row that is out lies in this wave's part
-            for (int64_t i0 = w_lo; i0 < w_hi; i0 += step) {
-                const int64_t i = i0 + lane * N;
-                uint32_t o[N];
-                r.load(i, o);
-                int cnt = 0;
+            for (int j = 0; j < AHEAD; ++j) {
+                const int i = t0 + j < to ? at(t0 + j) : src.vocab;
+                next[j] = src.load(i);
+                bits[j] = src.bits(i);
+            }
+        };
+        fetch(from);
+#pragma unroll 1
+        for (int t0 = from; t0 < to; t0 += AHEAD) {
+            Piece<T> now[AHEAD];
 #pragma unroll
-                for (int e = 0; e < N; ++e) cnt += o[e] == cut ? 1 : 0;
-                int inc = cnt;
+            for (int j = 0; j < AHEAD; ++j) {
+                now[j] = next[j];
+                src.finish(now[j], bits[j]);
+            }
+            fetch(t0 + AHEAD);
 #pragma unroll
-                for (int s = 1; s < 64; s <<= 1) {
-                    const int t = __shfl_up(inc, s);
-                    if (lane >= s) inc += t;
-                }
-                int64_t at = run + inc - cnt;
-                const bool here = at <= ties && at + cnt > ties;
-                if (here) {
-#pragma unroll
-                    for (int e = 0; e < N; ++e)
-                        if (o[e] == cut) {
-                            if (at == ties) chosen_above = (u64)(i + e);
-                            ++at;
-                        }
-                }
-                if (__ballot(here)) break;
-                run += __shfl(inc, 63);
+            for (int j = 0; j < AHEAD; ++j) {
+                __builtin_amdgcn_sched_barrier(0);
+                if (t0 + j < to) f(t0 + j, at(t0 + j), now[j]);
             }
         }
+    }
+    // every score, in no order: f(z)
+    template <class F> __device__ __forceinline__ void each(F&& f) const {
+        pieces(0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; }, [&](int, int, const Piece<T>& v) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) f(v.get(e));
+        });
+    }
+    // the steps [from, to) of the wave's share, in order: f(step, first element, piece)
+    template <class F> __device__ __forceinline__ void in_order(int from, int to, F&& f) const {
+        pieces(from, to, [&](int t) { return wave * share + (t * 64 + lane) * N; }, f);
+    }
+    // sh.part = the running sums of value(piece, first element) before each part; -> their sum
+    template <class Value> __device__ __forceinline__ u64 sum_parts(SampleShared& sh, Value&& value) const {
         __syncthreads();
-        tie_end = (int64_t)chosen_above;
-    }
-    auto remaining = [&](uint32_t o, int64_t i) -> u64 {
-        if (o == 0 || o < cut || (o == cut && i >= tie_end)) return 0;
-        if (use_min && weigh.exact(o) < least_w) return 0;
-        return weigh(o);
-    };
-    // weights by wave part, then the part and the row at which the running sum exceeds uniform * total
-    u64 mine = 0;
-    for (int64_t i = w_lo + lane * N; i < w_hi; i += step) {
-        uint32_t o[N];
-        r.load(i, o);
-#pragma unroll
-        for (int e = 0; e < N; ++e) mine += remaining(o[e], i + e);
-    }
-    mine = wave_sum(mine);
-    __syncthreads();
-    if (lane == 0) red[wave] = mine;
-    __syncthreads();
-    u64 total = 0, run = 0;
-    for (int w = 0; w < SAMPLE_WAVES; ++w) {
-        if (w < wave) run += red[w];
-        total += red[w];
-    }
-    // running sum > uniform * total, as integers: at least floor(uniform * total) + 1
-    const double goal = (double)a.uniform[row] * (double)total;
-    u64 least = goal >= 0.0 ? (u64)floor(goal) + 1 : 1;
-    if (!(least <= total)) least = total;
-    if (run < least && run + mine >= least) {
-        for (int64_t i0 = w_lo; i0 < w_hi; i0 += step) {
-            const int64_t i = i0 + lane * N;
-            uint32_t o[N];
-            r.load(i, o);
-            u64 w[N], sum = 0;
-#pragma unroll
-            for (int e = 0; e < N; ++e) sum += w[e] = remaining(o[e], i + e);
-            u64 inc = sum;
-#pragma unroll
-            for (int s = 1; s < 64; s <<= 1) {
-                const u64 t = __shfl_up(inc, s);
-                if (lane >= s) inc += t;
+        u64 sum = 0;
+        in_order(0, steps, [&](int t, int at, const Piece<T>& v) {
+            sum += value(v, at);
+            if ((t + 1) % per_group == 0 || t + 1 == steps) {
+                sum = wave_sum(sum);
+                if (lane == 0) sh.part[wave * groups + t / per_group] = sum;
+                sum = 0;
             }
-            u64 at = run + inc - sum;
-            const bool here = at < least && at + sum >= least;
-            if (here) {
+        });
+        return scan_parts(sh, parts);
+    }
+    // the parts of the wave that hold(sum before, sum up to): f(sum before, group)
+    template <class Hold, class F> __device__ __forceinline__ void parts_that(const SampleShared& sh, u64 total, Hold&& hold, F&& f) const {
+        for (int g = 0; g < groups; ++g) {
+            const int k = wave * groups + g;
+            const u64 from = sh.part[k], to = k + 1 < parts ? sh.part[k + 1] : total;
+            if (hold(from, to)) f(from, g);
+        }
+    }
+    // The scores at or above thr to the list, in row order; -> their number, nothing written where that exceeds LIST_MAX.
+    __device__ __forceinline__ int compact(SampleShared& sh, float thr) const {
+        auto count = [&](const Piece<T>& v) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) c += v.get(e) >= thr ? 1 : 0;
+            return c;
+        };
+        const u64 total = sum_parts(sh, [&](const Piece<T>& v, int) { return (u64)count(v); });
+        if (total > LIST_MAX) return LIST_MAX + 1;
+        parts_that(sh, total, [](u64 from, u64 to) { return from < to; }, [&](u64 before, int g) {
+            uint32_t from = (uint32_t)before;
+            in_order(g * per_group, min((g + 1) * per_group, steps), [&](int, int at, const Piece<T>& v) {
+                const uint32_t c = count(v);
+                const u64 inc = wave_scan(c);
+                uint32_t to = from + (uint32_t)inc - c;
 #pragma unroll
                 for (int e = 0; e < N; ++e) {
-                    if (at < least && at + w[e] >= least) {
-                        a.out_row[row] = i + e;
-                        if (a.out_logp) a.out_logp[row] = (float)log((double)w[e] / (double)total);
+                    const float z = v.get(e);
+                    if (z >= thr) {
+                        sh.list_z[to] = z;
+                        sh.list_at[to] = (uint32_t)(at + e);
+                        ++to;
                     }
-                    at += w[e];
                 }
+                from += (uint32_t)last_lane(inc);
+            });
+        });
+        __syncthreads();
+        return (int)total;
+    }
+};
+
+template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared& sh, const T* scores, const SampleArgs& a, int64_t row) {
+    constexpr int N = Piece<T>::N;
+    RowPasses<T> pass(Source<T>(scores, a, row));
+    const int tid = threadIdx.x, lane = pass.lane;
+    const Settings set(a, row);
+    make_table(sh.table, tid, SAMPLE_NT);
+    // ---- the largest score of each thread, and of the row
+    float mine = -INFINITY;
+    pass.each([&](float z) { mine = fmaxf(mine, z); });
+    float best = mine;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+    __syncthreads();
+    if (lane == 0) sh.red[pass.wave] = __float_as_uint(best);
+    if (tid == 0) sh.first = 0xffffffffu;
+    __syncthreads();
+    for (int w = 0; w < SAMPLE_WAVES; ++w) best = fmaxf(best, __uint_as_float((uint32_t)sh.red[w]));
+    if (best == -INFINITY) {
+        if (tid == 0) write_certain(a, row, -1);
+        return;
+    }
+    if (set.first_of_best()) {
+        uint32_t at = 0xffffffffu;
+        if (mine == best) {
+#pragma unroll 1
+            for (int i = tid * N; i < pass.src.vocab && at == 0xffffffffu; i += SAMPLE_NT * N) {
+                Piece<T> v = pass.src.load(i);
+                pass.src.finish(v, pass.src.bits(i));
+#pragma unroll
+                for (int e = N - 1; e >= 0; --e)
+                    if (v.get(e) == best) at = (uint32_t)(i + e);
             }
-            if (__ballot(here)) break;
-            run += __shfl(inc, 63);
+            atomicMin(&sh.first, at);
+        }
+        __syncthreads();
+        if (tid == 0) write_certain(a, row, sh.first);
+        return;
+    }
+    if (best == INFINITY) {
+        pass.src.infinite = true;
+        mine = mine == INFINITY ? 0.0f : -INFINITY;
+        best = 0.0f;
+    }
+    const FixedExp weigh(best, set.tau, a.shift, sh.table);
+    const u64 least_w = set.least_weight(a.shift);
+
+    // ---- few rows can remain: a list of them
+    float thr = -INFINITY;
+    if (set.by_count() && set.top_k <= SAMPLE_NT) {
+        u64 above;
+        const uint32_t o = narrow(sh, [&](auto&& f) { f(pattern(mine), one_each); }, 1u, pattern(best), 0, (u64)set.top_k, &above, 2);
+        thr = o > 0x00800000u ? score_of(o) : LOWEST;            // fewer than top_k threads hold anything: everything
+    } else if (!set.by_count() && !set.by_mass() && least_w) {
+        thr = set.min_p_bound(best);
+    }
+    if (thr > -INFINITY) {
+        const int listed = pass.compact(sh, thr);
+        if (listed <= LIST_MAX) return draw_listed(sh, a, row, set, weigh, listed);
+    }
+
+    // ---- the lowest score that remains (cut), and how many of the rows at it
+    float cut = -INFINITY;
+    int64_t ties = INT64_MAX;
+    // The score, from the best, at which the running sum of value(z) reaches target(total); false where scores that weigh
+    // anything do not reach it.
+    auto find_cut = [&](auto&& value, auto&& target, float* at, u64* above) {
+        clear_bins(sh);
+        u64 sum = 0;
+        pass.each([&](float z) {
+            if (z >= weigh.cut) {
+                const u64 v = value(z);
+                sum += v;
+                if (v) atomicAdd(&sh.bin[weigh.bin(z)], v);
+            }
+        });
+        const u64 least = target(block_total(sh, sum));
+        find_bin(sh, 0, least, false);
+        const int b = (int)sh.found;
+        if (b == BINS) return false;
+        const u64 before = sh.found_sum;
+        float lo, hi;
+        weigh.bin_range(b, &lo, &hi);
+        // the bin's scores go to the list, where they fit; else they are picked out of the row again in each step
+        __syncthreads();
+        if (tid == 0) sh.found = 0;
+        __syncthreads();
+        pass.each([&](float z) {
+            if (z < lo || z > hi || !(z >= weigh.cut) || weigh.bin(z) != b) return;
+            const uint32_t to = atomicAdd(&sh.found, 1u);
+            if (to < LIST_MAX) sh.list_z[to] = z;
+        });
+        __syncthreads();
+        const int members = (int)sh.found;
+        __syncthreads();
+        *at = score_of(narrow(sh, [&](auto&& f) {
+            if (members <= LIST_MAX) {
+                for (int i = tid; i < members; i += SAMPLE_NT) {
+                    const float z = sh.list_z[i];
+                    f(pattern(z), [&] { return value(z); });
+                }
+            } else {
+                pass.each([&](float z) {
+                    if (z >= lo && z <= hi && z >= weigh.cut && weigh.bin(z) == b) f(pattern(z), [&] { return value(z); });
+                });
+            }
+        }, pattern(lo), pattern(hi), before, least, above));
+        return true;
+    };
+    if (set.by_count()) {
+        u64 above;
+        float at;
+        if (find_cut([](float) { return (u64)1; }, [&](u64) { return (u64)set.top_k; }, &at, &above)) {
+            cut = at;
+            ties = set.top_k - (int64_t)above;
         }
     }
+    if (set.by_mass()) {
+        const float floor_z = cut;
+        const u64 w_cut = ties < INT64_MAX ? weigh(cut) : 0;
+        u64 above = 0, over = 0;
+        float at = 0.0f;
+        double target = 0.0;
+        if (find_cut([&](float z) { return z > floor_z ? weigh(z) : (u64)0; },
+                     [&](u64 total) {
+                         over = total;
+                         target = (double)(total + w_cut * (u64)(ties < INT64_MAX ? ties : 0)) * (double)set.top_p;
+                         return max((u64)ceil(target), (u64)1);
+                     },
+                     &at, &above)) {
+            cut = at;
+            ties = ties_within(target, above, weigh(at));
+        } else if (w_cut) {
+            ties = min(ties, ties_within(target, over, w_cut));
+        }
+    }
+
+    // ---- the draw
+    __syncthreads();
+    if (tid == 0) sh.first = 0xffffffffu;             // rows at the cut from this one on are out
+    if (ties < INT64_MAX) {
+        auto ties_in = [&](const Piece<T>& v) {
+            uint32_t c = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) c += v.get(e) == cut ? 1 : 0;
+            return c;
+        };
+        const u64 total = pass.sum_parts(sh, [&](const Piece<T>& v, int) { return (u64)ties_in(v); });
+        pass.parts_that(sh, total, [&](u64 from, u64 to) { return (int64_t)from <= ties && (int64_t)to > ties; }, [&](u64 before, int g) {
+            int64_t run = (int64_t)before;
+            pass.in_order(g * pass.per_group, min((g + 1) * pass.per_group, pass.steps), [&](int, int at, const Piece<T>& v) {
+                const uint32_t c = ties_in(v);
+                const u64 inc = wave_scan(c);
+                int64_t k = run + (int64_t)inc - c;
+#pragma unroll
+                for (int e = 0; e < N; ++e)
+                    if (v.get(e) == cut) {
+                        if (k == ties) sh.first = (uint32_t)(at + e);
+                        ++k;
+                    }
+                run += (int64_t)last_lane(inc);
+            });
+        });
+    }
+    __syncthreads();
+    const uint32_t tie_end = sh.first;
+    auto weight_at = [&](float z, uint32_t at) {
+        const u64 w = weigh(z);
+        return (z > cut || (z == cut && at < tie_end)) && w >= least_w ? w : (u64)0;
+    };
+    const u64 total = pass.sum_parts(sh, [&](const Piece<T>& v, int at) {
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += weight_at(v.get(e), (uint32_t)(at + e));
+        return sum;
+    });
+    const u64 least = set.goal(total);
+    pass.parts_that(sh, total, [&](u64 from, u64 to) { return from < least && to >= least; }, [&](u64 before, int g) {
+        u64 run = before;
+        pass.in_order(g * pass.per_group, min((g + 1) * pass.per_group, pass.steps), [&](int, int at, const Piece<T>& v) {
+            u64 w[N], sum = 0;
+#pragma unroll
+            for (int e = 0; e < N; ++e) sum += w[e] = weight_at(v.get(e), (uint32_t)(at + e));
+            const u64 inc = wave_scan(sum);
+            u64 k = run + inc - sum;
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                if (k < least && k + w[e] >= least) write_draw(a, row, (uint32_t)(at + e), w[e], total);
+                k += w[e];
+            }
+            run += last_lane(inc);
+        });
+    });
+}
+
+template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_kernel(const T* __restrict__ scores, SampleArgs a) {
+    __shared__ SampleShared sh;
+    sample_whole_row(sh, scores, a, blockIdx.x);
 }
 
 }  // namespace vdb
