@@ -702,6 +702,452 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_kernel(co
     sample_whole_row(sh, scores, a, blockIdx.x);
 }
 
+// ---------------------------------------------------------------- long rows, by the whole chip
+// 1 sample_groups: the maxima of groups of 32 scores (and the histograms cleared)
+// 2 sample_pick (a block per row): rows that the best score or a list settles are finished from the maxima and the few
+//   groups that reach the bound; the others are marked
+// 3 sample_weigh: marked rows' weights, by parts of the row, and by distance from the best where top-p asks for it
+// 4 sample_border (a block per row): the draw from the parts, or the bin in which the border of top-p lies
+// 5 sample_above: the weights above that bin by parts, and the bin's members
+// 6 sample_rest (a block per row): the border among the members and the draw; rows for which a list was too short go through
+//   all passes by one block
+static constexpr int GROUP = 32, STREAM_NT = 256, STREAM_PIECES = 4;
+enum RowMode { ROW_DONE = 0, ROW_WHOLE = 1, ROW_SUM = 2, ROW_MASS = 3 };
+struct RowState {
+    u64 above, least;                // weights above the bin of the border; the running sum that the border reaches
+    double target;
+    float best;
+    int mode, bin;
+    uint32_t members;
+};
+static constexpr int PARTS = SAMPLE_WAVES * GROUPS;                 // at most, per row
+struct SampleWork {
+    float* group_max; int groups;    // [n][groups]
+    RowState* state;                 // [n]
+    u64* hist;                       // [n][BINS]
+    u64* part; int parts, part_len;  // [n][PARTS], scores of a part (a multiple of 512)
+    float* member_z; uint32_t* member_at;                           // [n][LIST_MAX]
+    int64_t bytes;
+};
+static SampleWork sample_work(void* base, int64_t n, int64_t vocab) {
+    SampleWork w{};
+    char* at = (char*)base;
+    auto take = [&](int64_t bytes) {
+        char* here = at;
+        at += round_up64(bytes, 256);
+        return here;
+    };
+    w.groups = (int)((vocab + GROUP - 1) / GROUP);
+    w.part_len = (int)round_up64((vocab + PARTS - 1) / PARTS, 512);
+    w.parts = (int)((vocab + w.part_len - 1) / w.part_len);
+    w.group_max = (float*)take(n * w.groups * 4);
+    w.state = (RowState*)take(n * sizeof(RowState));
+    w.hist = (u64*)take(n * BINS * 8);
+    w.part = (u64*)take(n * PARTS * 8);
+    w.member_z = (float*)take(n * LIST_MAX * 4);
+    w.member_at = (uint32_t*)take(n * LIST_MAX * 4);
+    w.bytes = at - (char*)base;
+    return w;
+}
+
+template <class T>
+__global__ void __launch_bounds__(STREAM_NT) sample_groups_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork w, int slices) {
+    constexpr int N = Piece<T>::N;
+    const int64_t row = blockIdx.x / slices;
+    const int slice = (int)(blockIdx.x - row * slices);
+    const Source<T> src(scores, a, row);
+    Piece<T> x[STREAM_PIECES];
+    uint32_t bits[STREAM_PIECES];
+    const int first = (slice * STREAM_PIECES * STREAM_NT + (int)threadIdx.x) * N;
+#pragma unroll
+    for (int j = 0; j < STREAM_PIECES; ++j) {
+        x[j] = src.load(first + j * STREAM_NT * N);
+        bits[j] = src.bits(first + j * STREAM_NT * N);
+    }
+    for (int b = slice * STREAM_NT + threadIdx.x; b < BINS; b += slices * STREAM_NT) w.hist[row * BINS + b] = 0;
+    if (slice == 0 && threadIdx.x == 0) w.state[row] = RowState{};
+#pragma unroll
+    for (int j = 0; j < STREAM_PIECES; ++j) {
+        const int at = first + j * STREAM_NT * N;
+        src.finish(x[j], bits[j]);
+        float m = -INFINITY;
+#pragma unroll
+        for (int e = 0; e < N; ++e) m = fmaxf(m, x[j].get(e));
+        m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0xB1, 0xf, 0xf, false)));      // quad_perm:[1,0,3,2]
+        m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4E, 0xf, 0xf, false)));      // quad_perm:[2,3,0,1]
+        if (N == 4) m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x141, 0xf, 0xf, false)));   // row_half_mirror
+        if (threadIdx.x % (GROUP / N) == 0 && at < src.vocab) w.group_max[row * w.groups + at / GROUP] = m;
+    }
+}
+
+template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+    __shared__ SampleShared sh;
+    const int64_t row = blockIdx.x;
+    const Source<T> src(scores, a, row);
+    const Settings set(a, row);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const float* group_max = work.group_max + row * work.groups;
+    // a contiguous run of groups a thread
+    const int per = (work.groups + SAMPLE_NT - 1) / SAMPLE_NT, g0 = min(tid * per, work.groups), g1 = min(g0 + per, work.groups);
+    float best = -INFINITY;
+    for (int g = g0; g < g1; ++g) best = fmaxf(best, group_max[g]);
+    const float mine = best;
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
+    if (lane == 0) sh.red[wave] = __float_as_uint(best);
+    if (tid == 0) sh.first = 0xffffffffu;
+    make_table(sh.table, tid, SAMPLE_NT);
+    __syncthreads();
+    for (int v = 0; v < SAMPLE_WAVES; ++v) best = fmaxf(best, __uint_as_float((uint32_t)sh.red[v]));
+    if (best == -INFINITY) {
+        if (tid == 0) write_certain(a, row, -1);
+        return;
+    }
+    if (set.first_of_best()) {
+        if (mine == best) {
+            int g = g0;
+            while (group_max[g] != best) ++g;
+            atomicMin(&sh.first, (uint32_t)g);
+        }
+        __syncthreads();
+        if (tid < GROUP) {
+            const int at = (int)sh.first * GROUP + tid;
+            const unsigned long long m = __ballot(src.one(at) == best);
+            if (tid == 0) write_certain(a, row, (int64_t)sh.first * GROUP + __builtin_ctzll(m));
+        }
+        return;
+    }
+    const FixedExp weigh(best, set.tau, a.shift, sh.table);
+    float thr = -INFINITY;
+    int mode = best == INFINITY ? ROW_WHOLE : set.by_count() ? ROW_WHOLE : set.by_mass() ? ROW_MASS : ROW_SUM;
+    if (best < INFINITY) {
+        if (set.by_count() && set.top_k <= SAMPLE_NT) {
+            u64 above;
+            const uint32_t o = narrow(sh, [&](auto&& f) {
+                for (int g = g0; g < g1; ++g) f(pattern(group_max[g]), one_each);
+            }, 1u, pattern(best), 0, (u64)set.top_k, &above, 2);
+            thr = o > 0x00800000u ? score_of(o) : LOWEST;            // fewer than top_k groups hold anything: everything
+        } else if (!set.by_count() && !set.by_mass() && set.min_p > 0.0f) {
+            thr = set.min_p_bound(best);
+        }
+    }
+    if (thr > -INFINITY) {
+        // the groups that reach the bound, in order, where the list's rows go later
+        uint32_t count = 0;
+        for (int g = g0; g < g1; ++g) count += group_max[g] >= thr ? 1 : 0;
+        u64 found;
+        uint32_t to = (uint32_t)block_scan(sh, count, &found);
+        if (found <= LIST_MAX) {
+            uint32_t* group = (uint32_t*)sh.bin;
+            for (int g = g0; g < g1; ++g)
+                if (group_max[g] >= thr) group[to++] = (uint32_t)g;
+            __syncthreads();
+            // 64 scores a wave: two groups
+            const int chunks = ((int)found + 1) / 2;
+            auto score = [&](int c, int* at) {
+                const int k = 2 * c + (lane >> 5);
+                *at = k < (int)found ? (int)group[k] * GROUP + (lane & (GROUP - 1)) : src.vocab;
+                return src.one(*at);
+            };
+            for (int c = wave; c < chunks; c += SAMPLE_WAVES) {
+                int at;
+                const unsigned long long m = __ballot(score(c, &at) >= thr);
+                if (lane == 0) sh.part[c] = (u64)__popcll(m);
+            }
+            const u64 listed = scan_parts(sh, chunks);
+            if (listed <= LIST_MAX) {
+                for (int c = wave; c < chunks; c += SAMPLE_WAVES) {
+                    int at;
+                    const float z = score(c, &at);
+                    const unsigned long long m = __ballot(z >= thr);
+                    if (z >= thr) {
+                        const uint32_t i = (uint32_t)sh.part[c] + (uint32_t)__popcll(m & ((1ull << lane) - 1));
+                        sh.list_z[i] = z;
+                        sh.list_at[i] = (uint32_t)at;
+                    }
+                }
+                __syncthreads();
+                return draw_listed(sh, a, row, set, weigh, (int)listed);
+            }
+        }
+    }
+    if (tid == 0) {
+        work.state[row].best = best;
+        work.state[row].mode = mode;
+    }
+}
+
+// Parts [p0, p0 + count) of a row, one wave each after the other: f(piece, first element) is added up into work.part.
+template <class T, class F>
+__device__ __forceinline__ void stream_parts(const Source<T>& src, const SampleWork& work, int64_t row, int p0, int count, F&& f) {
+    constexpr int N = Piece<T>::N;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    for (int p = p0 + wave; p < min(p0 + count, work.parts); p += STREAM_NT / 64) {
+        u64 sum = 0;
+        const int end = (p + 1) * work.part_len;
+        for (int at0 = p * work.part_len; at0 < end; at0 += 512) {
+            Piece<T> x[512 / (64 * N)];
+            uint32_t bits[512 / (64 * N)];
+#pragma unroll
+            for (int j = 0; j < 512 / (64 * N); ++j) {
+                x[j] = src.load(at0 + (j * 64 + lane) * N);
+                bits[j] = src.bits(at0 + (j * 64 + lane) * N);
+            }
+#pragma unroll
+            for (int j = 0; j < 512 / (64 * N); ++j) {
+                src.finish(x[j], bits[j]);
+                sum += f(x[j], at0 + (j * 64 + lane) * N);
+            }
+        }
+        sum = wave_sum(sum);
+        if (lane == 0) work.part[row * PARTS + p] = sum;
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(STREAM_NT) sample_weigh_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int slices, int parts_each) {
+    constexpr int N = Piece<T>::N;
+    __shared__ double table[EXP_STEPS];
+    __shared__ u64 hist[BINS];
+    const int64_t row = blockIdx.x / slices;
+    const int slice = (int)(blockIdx.x - row * slices), mode = work.state[row].mode;
+    if (mode != ROW_SUM && mode != ROW_MASS) return;
+    const Source<T> src(scores, a, row);
+    const Settings set(a, row);
+    make_table(table, threadIdx.x, STREAM_NT);
+    if (mode == ROW_MASS)
+        for (int b = threadIdx.x; b < BINS; b += STREAM_NT) hist[b] = 0;
+    __syncthreads();
+    const FixedExp weigh(work.state[row].best, set.tau, a.shift, table);
+    const u64 least_w = mode == ROW_SUM ? set.least_weight(a.shift) : 0;
+    stream_parts(src, work, row, slice * parts_each, parts_each, [&](const Piece<T>& v, int) {
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float z = v.get(e);
+            const u64 w = weigh(z);
+            sum += w >= least_w ? w : 0;
+            if (mode == ROW_MASS && w) atomicAdd(&hist[weigh.bin(z)], w);
+        }
+        return sum;
+    });
+    if (mode != ROW_MASS) return;
+    __syncthreads();
+    for (int b = threadIdx.x; b < BINS; b += STREAM_NT)
+        if (hist[b]) atomicAdd(&work.hist[row * BINS + b], hist[b]);
+}
+
+// The row's parts, of `total` after scan_parts: the one that holds the goal, read again by the first wave.
+template <class T, class Weight>
+__device__ __forceinline__ void draw_from_parts(SampleShared& sh, const Source<T>& src, const SampleArgs& a, const SampleWork& work, int64_t row,
+                                                const Settings& set, u64 total, Weight&& weight_at) {
+    constexpr int N = Piece<T>::N;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const u64 least = set.goal(total);
+    if (tid < work.parts) {
+        const u64 from = sh.part[tid], to = tid + 1 < work.parts ? sh.part[tid + 1] : total;
+        if (from < least && to >= least) {
+            sh.found = (uint32_t)tid;
+            sh.found_sum = from;
+        }
+    }
+    __syncthreads();
+    if (tid >= 64) return;
+    u64 run = sh.found_sum;
+    const int start = (int)sh.found * work.part_len, end = start + work.part_len;
+    for (int at0 = start; at0 < end && run < least; at0 += 64 * N) {
+        const int at = at0 + lane * N;
+        Piece<T> v = src.load(at);
+        src.finish(v, src.bits(at));
+        u64 w[N], sum = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += w[e] = weight_at(v.get(e), (uint32_t)(at + e));
+        const u64 inc = wave_scan(sum);
+        u64 k = run + inc - sum;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            if (k < least && k + w[e] >= least) write_draw(a, row, (uint32_t)(at + e), w[e], total);
+            k += w[e];
+        }
+        run += last_lane(inc);
+    }
+}
+
+template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_border_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+    __shared__ SampleShared sh;
+    const int64_t row = blockIdx.x;
+    RowState& state = work.state[row];
+    const int mode = state.mode, tid = threadIdx.x;
+    if (mode != ROW_SUM && mode != ROW_MASS) return;
+    const Settings set(a, row);
+    if (tid < work.parts) sh.part[tid] = work.part[row * PARTS + tid];
+    if (mode == ROW_MASS) {
+        for (int b = tid; b < BINS; b += SAMPLE_NT) sh.bin[b] = work.hist[row * BINS + b];
+        const u64 total = block_total(sh, tid < work.parts ? sh.part[tid] : 0);
+        const double target = (double)total * (double)set.top_p;
+        const u64 least = max((u64)ceil(target), (u64)1);
+        find_bin(sh, 0, least, false);
+        if (tid == 0) {
+            state.above = sh.found_sum;
+            state.least = least;
+            state.target = target;
+            state.bin = (int)sh.found;
+        }
+        return;
+    }
+    make_table(sh.table, tid, SAMPLE_NT);
+    const u64 total = scan_parts(sh, work.parts), least_w = set.least_weight(a.shift);
+    const FixedExp weigh(state.best, set.tau, a.shift, sh.table);
+    draw_from_parts(sh, Source<T>(scores, a, row), a, work, row, set, total, [&](float z, uint32_t) {
+        const u64 w = weigh(z);
+        return w >= least_w ? w : (u64)0;
+    });
+}
+
+template <class T>
+__global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int slices, int parts_each) {
+    constexpr int N = Piece<T>::N;
+    __shared__ double table[EXP_STEPS];
+    const int64_t row = blockIdx.x / slices;
+    const int slice = (int)(blockIdx.x - row * slices);
+    RowState& state = work.state[row];
+    if (state.mode != ROW_MASS) return;
+    const Source<T> src(scores, a, row);
+    const Settings set(a, row);
+    make_table(table, threadIdx.x, STREAM_NT);
+    __syncthreads();
+    const FixedExp weigh(state.best, set.tau, a.shift, table);
+    const u64 least_w = set.least_weight(a.shift);
+    const int b = state.bin;
+    float lo, hi;
+    weigh.bin_range(b, &lo, &hi);
+    stream_parts(src, work, row, slice * parts_each, parts_each, [&](const Piece<T>& v, int at) {
+        u64 sum = 0;
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float z = v.get(e);
+            if (!__ballot(z >= lo)) continue;
+            const int bin = z >= weigh.cut ? weigh.bin(z) : BINS;
+            if (bin < b) {
+                const u64 w = weigh(z);
+                sum += w >= least_w ? w : 0;
+            } else if (bin == b) {
+                const uint32_t to = atomicAdd(&state.members, 1u);
+                if (to < LIST_MAX) {
+                    work.member_z[row * LIST_MAX + to] = z;
+                    work.member_at[row * LIST_MAX + to] = (uint32_t)(at + e);
+                }
+            }
+        }
+        return sum;
+    });
+}
+
+template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_rest_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+    __shared__ SampleShared sh;
+    const int64_t row = blockIdx.x;
+    const RowState state = work.state[row];
+    const int tid = threadIdx.x;
+    if (state.mode == ROW_WHOLE || (state.mode == ROW_MASS && state.members > LIST_MAX)) return sample_whole_row(sh, scores, a, row);
+    if (state.mode != ROW_MASS) return;
+    const Settings set(a, row);
+    const int members = (int)state.members;
+    make_table(sh.table, tid, SAMPLE_NT);
+    for (int i = tid; i < members; i += SAMPLE_NT) {
+        sh.list_z[i] = work.member_z[row * LIST_MAX + i];
+        sh.list_at[i] = work.member_at[row * LIST_MAX + i];
+    }
+    if (tid < work.parts) sh.part[tid] = work.part[row * PARTS + tid];
+    if (tid == 0) sh.first = 0xffffffffu;
+    __syncthreads();
+    const FixedExp weigh(state.best, set.tau, a.shift, sh.table);
+    const u64 least_w = set.least_weight(a.shift);
+    float lo, hi;
+    weigh.bin_range(state.bin, &lo, &hi);
+    u64 above;
+    const float cut = score_of(narrow(sh, [&](auto&& f) {
+        for (int i = tid; i < members; i += SAMPLE_NT) {
+            const float z = sh.list_z[i];
+            f(pattern(z), [&] { return weigh(z); });
+        }
+    }, pattern(lo), pattern(hi), state.above, state.least, &above));
+    const int64_t ties = ties_within(state.target, above, weigh(cut));
+    u64 at_cut = 0;
+    for (int i = tid; i < members; i += SAMPLE_NT) at_cut += sh.list_z[i] == cut ? 1 : 0;
+    uint32_t tie_end = 0xffffffffu;              // rows at the cut from this one on are out
+    if ((int64_t)block_total(sh, at_cut) > ties) {
+        u64 ignored;
+        tie_end = ~narrow(sh, [&](auto&& f) {
+            for (int i = tid; i < members; i += SAMPLE_NT)
+                if (sh.list_z[i] == cut) f(~sh.list_at[i], one_each);
+        }, ~(uint32_t)a.vocab, 0xffffffffu, 0, (u64)ties + 1, &ignored);
+    }
+    auto weight_at = [&](float z, uint32_t at) {
+        const u64 w = weigh(z);
+        return (z > cut || (z == cut && at < tie_end)) && w >= least_w ? w : (u64)0;
+    };
+    __syncthreads();
+    for (int i = tid; i < members; i += SAMPLE_NT) {
+        const u64 w = weight_at(sh.list_z[i], sh.list_at[i]);
+        if (w) atomicAdd(&sh.part[sh.list_at[i] / (uint32_t)work.part_len], w);
+    }
+    const u64 total = scan_parts(sh, work.parts);
+    draw_from_parts(sh, Source<T>(scores, a, row), a, work, row, set, total, weight_at);
+}
+
+// Short rows go to one block each: what the other form saves in passes it loses in launches.
+static bool by_whole_chip(int64_t vocab) { return vocab >= 16384; }
+static const int64_t SAMPLE_BATCH = 1024;           // rows at a time by the whole chip: bounds the workspace (56 MB at 131072 scores)
+
+template <class T> static int launch_long_rows(const T* z, int64_t n, const SampleArgs& a, const SampleWork& w, hipStream_t s) {
+    const dim3 rows((unsigned)n), block(SAMPLE_NT);
+    const int slices = ceil_div(a.vocab, STREAM_NT * Piece<T>::N * STREAM_PIECES);
+    hipLaunchKernelGGL(sample_groups_kernel<T>, dim3((unsigned)(n * slices)), dim3(STREAM_NT), 0, s, z, a, w, slices);
+    VDB_HIP(hipGetLastError());
+    hipLaunchKernelGGL(sample_pick_kernel<T>, rows, block, 0, s, z, a, w);
+    VDB_HIP(hipGetLastError());
+    const bool settled = (!a.d_temperature && !(a.temperature > 0.0f)) || (!a.d_top_p && a.top_p <= 0.0f) ||
+                         (!a.d_top_k && a.top_k >= 1 && a.top_k <= SAMPLE_NT);      // whatever the scores, but for long ties
+    if (!settled) {
+        // parts a block: few where there are few rows, so that they spread over the chip, else enough to pay for its table
+        const int parts_each = n * w.parts >= (int64_t)2048 * 32 ? 32 : 8, cuts = ceil_div(w.parts, parts_each);
+        const dim3 grid((unsigned)(n * cuts));
+        hipLaunchKernelGGL(sample_weigh_kernel<T>, grid, dim3(STREAM_NT), 0, s, z, a, w, cuts, parts_each);
+        VDB_HIP(hipGetLastError());
+        hipLaunchKernelGGL(sample_border_kernel<T>, rows, block, 0, s, z, a, w);
+        VDB_HIP(hipGetLastError());
+        if (a.d_top_p || a.top_p < 1.0f) {
+            hipLaunchKernelGGL(sample_above_kernel<T>, grid, dim3(STREAM_NT), 0, s, z, a, w, cuts, parts_each);
+            VDB_HIP(hipGetLastError());
+        }
+    }
+    hipLaunchKernelGGL(sample_rest_kernel<T>, rows, block, 0, s, z, a, w);
+    VDB_HIP(hipGetLastError());
+    return VDB_OK;
+}
+
+template <class T> static int launch_sample(const T* z, int64_t n, const SampleArgs& a, void* d_work, hipStream_t s) {
+    if (!by_whole_chip(a.vocab)) {
+        hipLaunchKernelGGL(sample_kernel<T>, dim3((unsigned)n), dim3(SAMPLE_NT), 0, s, z, a);
+        VDB_HIP(hipGetLastError());
+        return VDB_OK;
+    }
+    const SampleWork w = sample_work(d_work, std::min(n, SAMPLE_BATCH), a.vocab);
+    for (int64_t r = 0; r < n; r += SAMPLE_BATCH) {
+        SampleArgs b = a;
+        b.uniform += r;
+        if (b.d_temperature) b.d_temperature += r;
+        if (b.d_top_k) b.d_top_k += r;
+        if (b.d_top_p) b.d_top_p += r;
+        if (b.d_min_p) b.d_min_p += r;
+        if (b.mask) b.mask += r * b.mask_ld;
+        b.out_row += r;
+        if (b.out_logp) b.out_logp += r;
+        VDB_TRY(launch_long_rows(z + r * a.ld, std::min(n - r, SAMPLE_BATCH), b, w, s));
+    }
+    return VDB_OK;
+}
+
 }  // namespace vdb
 
 using namespace vdb;
@@ -710,7 +1156,7 @@ int vdb_sample_workspace(int64_t n, int64_t vocab, int64_t* bytes) {
     VDB_REQUIRE(bytes, "null pointer for the workspace size");
     VDB_REQUIRE(n >= 0 && vocab >= 1 && vocab <= ((int64_t)1 << 24), "bad sizes for sampling: %lld rows of %lld scores (at most 2^24)", (long long)n,
                 (long long)vocab);
-    *bytes = 0;
+    *bytes = by_whole_chip(vocab) ? sample_work(nullptr, std::min(n, SAMPLE_BATCH), vocab).bytes : 0;
     return VDB_OK;
 }
 
@@ -736,8 +1182,6 @@ int vdb_sample_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int
                        d_mask, mask_ld, d_out_row, d_out_logp, std::min(52, 62 - bits)};
     return with_type(type, [&](auto* p) -> int {
         typedef std::remove_pointer_t<decltype(p)> T;
-        hipLaunchKernelGGL(sample_kernel<T>, dim3((unsigned)n), dim3(SAMPLE_NT), 0, (hipStream_t)stream, (const T*)d_scores, a);
-        VDB_HIP(hipGetLastError());
-        return VDB_OK;
+        return launch_sample((const T*)d_scores, n, a, d_work, (hipStream_t)stream);
     });
 }
