@@ -21,6 +21,7 @@ are taken in 32 bits or more, and equal inputs give equal bits.  Arguments that 
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import Optional, Tuple, Union
 
 import torch
@@ -29,14 +30,22 @@ from . import _native
 
 VALUE_TYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
+# What a call needs of the library and the device, looked up once: small calls are bound by what happens on the host.
+_lib = None
+_device_no = -1
+_where: Optional[torch.device] = None
+
 
 def _fail(text: str):
     raise ValueError(text)
 
 
-def _device() -> int:
+def _start() -> None:
+    global _lib, _device_no, _where
     _native.init()
-    return _native.current_device() or 0
+    _device_no = _native.current_device() or 0
+    _where = torch.device("cuda", _device_no)
+    _lib = _native.load()
 
 
 def _on_gpu(t, what: str) -> None:
@@ -44,21 +53,25 @@ def _on_gpu(t, what: str) -> None:
         _fail(f"{what} must be a torch tensor, got {type(t).__name__}")
     if not t.is_cuda:
         _fail(f"{what} must be on the GPU, it is on {t.device}")
-    if t.device.index != _device():
-        _fail(f"{what} must be on GPU {_device()}, the library's device; it is on {t.device}")
+    if _lib is None:
+        _start()
+    if t.get_device() != _device_no:
+        _fail(f"{what} must be on GPU {_device_no}, the library's device; it is on {t.device}")
 
 
 def _matrix(t, what: str) -> Tuple[int, int, int, int]:
     """(value type, rows, columns, leading dimension) of a matrix whose rows are contiguous."""
     _on_gpu(t, what)
-    if t.dtype not in VALUE_TYPES:
+    code = VALUE_TYPES.get(t.dtype)
+    if code is None:
         _fail(f"{what} must be float32, bfloat16 or float16, got {t.dtype}")
     if t.dim() != 2:
         _fail(f"{what} must have two dimensions, got shape {tuple(t.shape)}")
     n, d = t.shape
-    if d > 1 and n > 0 and t.stride(1) != 1:
+    ld, step = t.stride()
+    if step != 1 and d > 1 and n > 0:
         _fail(f"the rows of {what} must be contiguous, its strides are {t.stride()}")
-    return VALUE_TYPES[t.dtype], n, d, t.stride(0) if n > 1 else d
+    return code, n, d, ld if n > 1 else d
 
 
 def _vector(t, what: str, n: int, dtype: torch.dtype) -> None:
@@ -74,10 +87,10 @@ def _row_numbers(t, what: str) -> torch.Tensor:
     return t
 
 
-def _output(out, what: str, shape, dtype: torch.dtype, inputs=()) -> torch.Tensor:
+def _output(out, what: str, shape, dtype: torch.dtype) -> torch.Tensor:
     """A new contiguous output, or the caller's, whose rows must not share memory."""
     if out is None:
-        return torch.empty(shape, device=f"cuda:{_device()}", dtype=dtype)
+        return torch.empty(shape, device=_where, dtype=dtype)
     _on_gpu(out, what)
     if out.dtype != dtype or tuple(out.shape) != tuple(shape):
         _fail(f"{what} must be {dtype} of shape {tuple(shape)}, got {out.dtype} of shape {tuple(out.shape)}")
@@ -87,17 +100,33 @@ def _output(out, what: str, shape, dtype: torch.dtype, inputs=()) -> torch.Tenso
 
 
 def _p(t: Optional[torch.Tensor]):
-    return None if t is None else C.c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
-def _stream():
-    return C.c_void_p(torch.cuda.current_stream(_device()).cuda_stream)
+def _stream() -> int:
+    return torch.cuda.current_stream(_device_no).cuda_stream
+
+
+_current_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+if _current_raw_stream is not None:
+    def _stream() -> int:                                   # noqa: F811 - the same number without a Stream object around it
+        return _current_raw_stream(_device_no)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(fn: str, *sizes) -> int:
+    need = C.c_int64(0)
+    _native.check(getattr(_native.load(), fn)(*sizes, C.byref(need)))
+    return need.value
 
 
 def _workspace(fn: str, *sizes):
-    need = C.c_int64(0)
-    _native.check(getattr(_native.load(), fn)(*sizes, C.byref(need)))
-    return torch.empty(need.value, device=f"cuda:{_device()}", dtype=torch.uint8) if need.value else None, need.value
+    """(tensor that holds the workspace, its address, its size); the tensor may be dropped once the call is enqueued."""
+    need = _workspace_bytes(fn, *sizes)
+    if not need:
+        return None, None, 0
+    t = torch.empty(need, device=_where, dtype=torch.uint8)
+    return t, t.data_ptr(), need
 
 
 # ---------------------------------------------------------------- lookup
@@ -109,7 +138,6 @@ def lookup(table: Union[torch.Tensor, "_native.RowStore"], rows: torch.Tensor, s
     n = rows.numel()
     store = table if isinstance(table, _native.RowStore) else None
     if store is not None:
-        _device()
         dim, natural = store.dim, torch.float32
     else:
         code, n_rows, dim, ld = _matrix(table, "table")
@@ -124,11 +152,10 @@ def lookup(table: Union[torch.Tensor, "_native.RowStore"], rows: torch.Tensor, s
     if out.dim() != 2 and not out.is_contiguous():
         _fail("out must be contiguous unless rows is a vector")
     ld_out = out.stride(0) if out.dim() == 2 and n > 1 else dim
-    lib = _native.load()
     if store is not None:
-        _native.check(lib.vdb_rows_lookup_dev(store.h, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], ld_out, _stream()))
+        _native.check(_lib.vdb_rows_lookup_dev(store.h, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], ld_out, _stream()))
     else:
-        _native.check(lib.vdb_lookup_dev(_p(table), code, n_rows, dim, ld, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], ld_out, _stream()))
+        _native.check(_lib.vdb_lookup_dev(_p(table), code, n_rows, dim, ld, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], ld_out, _stream()))
     return out
 
 
@@ -154,9 +181,9 @@ def lookup_grad(grad: torch.Tensor, rows: torch.Tensor, n_rows: int, scale: floa
     if dtype not in VALUE_TYPES:
         _fail(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     out = _output(out, "out", (n_rows, dim), dtype)
-    work, size = _workspace("vdb_lookup_grad_workspace", n, n_rows, dim)
-    _native.check(_native.load().vdb_lookup_grad_dev(_p(grad), code, ld, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], n_rows, dim,
-                                                     out.stride(0) if n_rows > 1 else dim, int(accumulate), _p(work), size, _stream()))
+    keep, work, size = _workspace("vdb_lookup_grad_workspace", n, n_rows, dim)
+    _native.check(_lib.vdb_lookup_grad_dev(_p(grad), code, ld, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], n_rows, dim,
+                                                     out.stride(0) if n_rows > 1 else dim, int(accumulate), work, size, _stream()))
     return out
 
 
@@ -192,10 +219,10 @@ def distill(scores: torch.Tensor, teacher: torch.Tensor, rows: torch.Tensor, tem
     ``distill_grad`` needs of this pass."""
     args = _distill_args(scores, teacher, rows, temperature, teacher_lse)
     n, vocab = scores.shape
-    loss = torch.empty(n, device=scores.device, dtype=torch.float32)
-    stats = torch.empty((n, 2), device=scores.device, dtype=torch.float32)
-    work, size = _workspace("vdb_distill_workspace", n, vocab)
-    _native.check(_native.load().vdb_distill_dev(*args, _p(loss), _p(stats), _p(work), size, _stream()))
+    loss = torch.empty(n, device=_where, dtype=torch.float32)
+    stats = torch.empty((n, 2), device=_where, dtype=torch.float32)
+    keep, work, size = _workspace("vdb_distill_workspace", n, vocab)
+    _native.check(_lib.vdb_distill_dev(*args, _p(loss), _p(stats), work, size, _stream()))
     return loss, stats
 
 
@@ -210,7 +237,7 @@ def distill_grad(scores: torch.Tensor, teacher: torch.Tensor, rows: torch.Tensor
         _fail(f"stats must be contiguous float32 of shape ({n}, 2), got {stats.dtype} of shape {tuple(stats.shape)}")
     _vector(grad_loss, "grad_loss", n, torch.float32)
     out = _output(out, "out", (n, vocab), scores.dtype)
-    _native.check(_native.load().vdb_distill_grad_dev(*args, _p(stats), _p(grad_loss), _p(out), out.stride(0) if n > 1 else vocab, _stream()))
+    _native.check(_lib.vdb_distill_grad_dev(*args, _p(stats), _p(grad_loss), _p(out), out.stride(0) if n > 1 else vocab, _stream()))
     return out
 
 
@@ -220,11 +247,11 @@ def distill_step(scores: torch.Tensor, teacher: torch.Tensor, rows: torch.Tensor
     args = _distill_args(scores, teacher, rows, temperature, teacher_lse)
     n, vocab = scores.shape
     _vector(grad_loss, "grad_loss", n, torch.float32)
-    loss = torch.empty(n, device=scores.device, dtype=torch.float32)
+    loss = torch.empty(n, device=_where, dtype=torch.float32)
     out = _output(out, "out", (n, vocab), scores.dtype)
-    work, size = _workspace("vdb_distill_workspace", n, vocab)
-    _native.check(_native.load().vdb_distill_step_dev(*args, _p(grad_loss), _p(loss), None, _p(out), out.stride(0) if n > 1 else vocab,
-                                                      _p(work), size, _stream()))
+    keep, work, size = _workspace("vdb_distill_workspace", n, vocab)
+    _native.check(_lib.vdb_distill_step_dev(*args, _p(grad_loss), _p(loss), None, _p(out), out.stride(0) if n > 1 else vocab,
+                                                      work, size, _stream()))
     return loss, out
 
 
@@ -272,9 +299,9 @@ def sample(scores: torch.Tensor, uniforms: torch.Tensor, temperature: Union[floa
             _fail(f"a filter over {vocab} scores takes {words} contiguous 32-bit words, for all rows or for each of {n}; got "
                   f"{mask_words.dtype} of shape {tuple(mask_words.shape)}")
         mask_ld = mask_words.stride(0) if mask_words.dim() == 2 and n > 1 else 0
-    out = torch.empty(n, device=scores.device, dtype=torch.int64)
-    logp = torch.empty(n, device=scores.device, dtype=torch.float32)
-    work, size = _workspace("vdb_sample_workspace", n, vocab)
-    _native.check(_native.load().vdb_sample_dev(_p(scores), code, n, vocab, ld, int(distances), _p(uniforms), t, tv, k, kv, p, pv, m, mv,
-                                                _p(mask_words), mask_ld, _p(out), _p(logp), _p(work), size, _stream()))
+    out = torch.empty(n, device=_where, dtype=torch.int64)
+    logp = torch.empty(n, device=_where, dtype=torch.float32)
+    keep, work, size = _workspace("vdb_sample_workspace", n, vocab)
+    _native.check(_lib.vdb_sample_dev(_p(scores), code, n, vocab, ld, int(distances), _p(uniforms), t, tv, k, kv, p, pv, m, mv,
+                                                _p(mask_words), mask_ld, _p(out), _p(logp), work, size, _stream()))
     return out, logp
