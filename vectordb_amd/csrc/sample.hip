@@ -21,7 +21,7 @@
 namespace vdb {
 
 static constexpr int SAMPLE_NT = 1024, SAMPLE_WAVES = SAMPLE_NT / 64;
-static constexpr int LIST_MAX = 2048, LIST_ITEMS = LIST_MAX / SAMPLE_NT, BINS = 2 * SAMPLE_NT, EXP_STEPS = 1024, GROUPS = 64, AHEAD = 4;
+static constexpr int LIST_MAX = 2048, LIST_ITEMS = LIST_MAX / SAMPLE_NT, BINS = 2 * SAMPLE_NT, EXP_STEPS = 1024, GROUPS = 64, AHEAD = 4, PAIRS = 256;
 typedef unsigned long long u64;
 static constexpr float LOWEST = -3.4028234663852886e38f;
 
@@ -146,6 +146,11 @@ struct FixedExp {
         const int k = (int)(uint32_t)__double_as_longlong(fma((double)z - best, c, NEAREST));
         return min((-k) >> 5, BINS - 1);
     }
+    // the same without the table, for a few scores: exp2() to the last bits of a double
+    __device__ __forceinline__ u64 directly(float z) const {
+        const double w = exp2(((double)z - best) * (c / EXP_STEPS));
+        return z >= cut ? (u64)__double_as_longlong(w + round_to) - (u64)__double_as_longlong(round_to) : 0;
+    }
     __device__ __forceinline__ u64 operator()(float z) const {
         constexpr double L = 0.69314718055994530942 / EXP_STEPS;
         const double d = (double)z - best;
@@ -168,11 +173,13 @@ struct SampleShared {
     float list_z[LIST_MAX];
     uint32_t list_at[LIST_MAX];
     u64 part[SAMPLE_WAVES * GROUPS];     // per part of the row, in row order: counts or weights, then their exclusive prefix
-    u64 before[256];
-    uint32_t rank[256];
+    u64 pair_sum[PAIRS], pair_w[PAIRS];
+    uint32_t pair_rank[PAIRS];
+    u64 few_w[64];
+    uint32_t few_key[64];
     u64 red[SAMPLE_WAVES];
     u64 found_sum;
-    uint32_t found, first;
+    uint32_t found, first, listed, few;
 };
 
 // Sums over a wave by data-parallel moves (rows of 16 lanes, then their last lanes passed on): a shuffle through LDS costs
@@ -254,32 +261,104 @@ __device__ static void find_bin(SampleShared& sh, u64 above, u64 target, bool fr
     __syncthreads();
 }
 
-// The key, among those of each(f) in [lo, hi], at which the running sum of the weights, from the top and from `above`, reaches
-// target (0 < target; where it is not reached: lo); *sum_above = the sum before it.  each calls f(key, weight), weight a
-// function.  11 bits a step; after fewer steps than the range has bits, the smallest key that can still be it.
+// 11 bits of a search: the part of [*lo, *hi] in which the running sum of the weights, by descending key and from *above,
+// reaches target (false: it does not; nothing changes).  each calls f(key, weight), weight a function.
 template <class Each>
-__device__ __forceinline__ uint32_t narrow(SampleShared& sh, Each&& each, uint32_t lo, uint32_t hi, u64 above, u64 target, u64* sum_above, int steps = 3) {
-    for (; steps > 0 && lo < hi; --steps) {
-        const int shift = max(21 - __clz(hi - lo), 0);
-        clear_bins(sh);
+__device__ __forceinline__ bool narrow_step(SampleShared& sh, Each&& each, uint32_t* lo, uint32_t* hi, u64* above, u64 target) {
+    const uint32_t first = *lo, last = *hi;
+    const int shift = max(21 - __clz(last - first), 0);
+    clear_bins(sh);
+    each([&](uint32_t key, auto&& weight) {
+        if (key < first || key > last) return;
+        const u64 v = weight();
+        if (v) atomicAdd(&sh.bin[(key - first) >> shift], v);
+    });
+    find_bin(sh, *above, target, true);
+    if (sh.found == BINS) return false;
+    const uint32_t b = BINS - 1 - sh.found, end = first + ((b + 1) << shift) - 1;
+    *above = sh.found_sum;
+    *lo = first + (b << shift);
+    if (end < last) *hi = end;
+    return true;
+}
+// The key among those of each(f) in [lo, hi] at which the running sum of the weights, by descending key and from `above`,
+// reaches target (0 < target; where it is not reached: lo); *sum_above = the sum before it.  What a step leaves is settled at
+// once by a wave that compares all pairs, if it is few.
+template <class Each>
+__device__ __forceinline__ uint32_t narrow(SampleShared& sh, Each&& each, uint32_t lo, uint32_t hi, u64 above, u64 target, u64* sum_above) {
+    while (lo < hi && narrow_step(sh, each, &lo, &hi, &above, target) && lo < hi) {
+        if (threadIdx.x == 0) sh.few = 0;
+        __syncthreads();
         each([&](uint32_t key, auto&& weight) {
             if (key < lo || key > hi) return;
             const u64 v = weight();
-            if (v) atomicAdd(&sh.bin[(key - lo) >> shift], v);
+            if (!v) return;
+            const uint32_t i = atomicAdd(&sh.few, 1u);
+            if (i < 64) { sh.few_key[i] = key; sh.few_w[i] = v; }
         });
-        find_bin(sh, above, target, true);
-        const uint32_t found = sh.found;
-        if (found == BINS) break;
-        const uint32_t b = BINS - 1 - found;
-        above = sh.found_sum;
-        const uint32_t last = lo + ((b + 1) << shift) - 1;
-        if (last < hi) hi = last;
-        lo += b << shift;
+        __syncthreads();
+        const uint32_t few = sh.few;
+        if (few <= 64) {
+            if (threadIdx.x < few) {
+                const uint32_t key = sh.few_key[threadIdx.x];
+                u64 before = above, upto = above;
+                for (uint32_t j = 0; j < few; ++j) {
+                    const u64 v = sh.few_w[j];
+                    if (sh.few_key[j] > key) before += v;
+                    if (sh.few_key[j] >= key) upto += v;
+                }
+                if (before < target && upto >= target) {         // equal keys write the same
+                    sh.found = key;
+                    sh.found_sum = before;
+                }
+            }
+            __syncthreads();
+            lo = sh.found;
+            above = sh.found_sum;
+            break;
+        }
     }
     *sum_above = above;
     return lo;
 }
 __device__ __forceinline__ u64 one_each() { return 1; }
+// A bound that no fewer than k of the scores of each(f) reach, and few more: the lower end of the part in which the k-th
+// largest lies.  lowest, best: their range.  -LOWEST where there are fewer than k.
+template <class Each> __device__ __forceinline__ float bound_of(SampleShared& sh, Each&& each, float lowest, float best, int k) {
+    uint32_t lo = pattern(lowest), hi = pattern(best);
+    u64 above = 0;
+    if (!narrow_step(sh, each, &lo, &hi, &above, (u64)k)) return LOWEST;
+    if (hi - lo >= 1u << 16) narrow_step(sh, each, &lo, &hi, &above, (u64)k);        // a range around zero holds most patterns
+    return score_of(lo);
+}
+// lanes with `want` add to the list; the number of all that wanted is in sh.listed
+__device__ __forceinline__ void append(SampleShared& sh, bool want, float z, uint32_t at) {
+    const unsigned long long m = __ballot(want);
+    if (!m) return;
+    const int lane = threadIdx.x & 63;
+    uint32_t from = 0;
+    if (lane == 0) from = atomicAdd(&sh.listed, (uint32_t)__popcll(m));
+    from = (uint32_t)__builtin_amdgcn_readfirstlane((int)from) + (uint32_t)__popcll(m & ((1ull << lane) - 1));
+    if (want && from < LIST_MAX) {
+        sh.list_z[from] = z;
+        sh.list_at[from] = at;
+    }
+}
+// smallest and largest over the block (-inf: nothing there), of values that are not NaN
+__device__ __forceinline__ void block_range(SampleShared& sh, float& lowest, float& best) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        best = fmaxf(best, __shfl_xor(best, o));
+        lowest = fminf(lowest, __shfl_xor(lowest, o));
+    }
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = ((u64)__float_as_uint(lowest) << 32) | __float_as_uint(best);
+    __syncthreads();
+    for (int w = 0; w < SAMPLE_WAVES; ++w) {
+        best = fmaxf(best, __uint_as_float((uint32_t)sh.red[w]));
+        lowest = fminf(lowest, __uint_as_float((uint32_t)(sh.red[w] >> 32)));
+    }
+}
 
 __device__ __forceinline__ void write_draw(const SampleArgs& a, int64_t row, uint32_t at, u64 w, u64 total) {
     a.out_row[row] = at;
@@ -294,101 +373,139 @@ __device__ __forceinline__ int64_t ties_within(double target, u64 above, u64 w) 
     return max((int64_t)1, (int64_t)ceil((target - (double)above) / (double)w));
 }
 
+// Of the rows at a cut, each(f) calling f(row), the first `ties` remain: the first one that is out (or 2^32 - 1).
+template <class Each> __device__ __forceinline__ uint32_t first_tie_out(SampleShared& sh, Each&& each, int64_t ties, uint32_t vocab) {
+    if (ties == INT64_MAX) return 0xffffffffu;
+    u64 count = 0, ignored;
+    each([&](uint32_t) { ++count; });
+    if ((int64_t)block_total(sh, count) <= ties) return 0xffffffffu;
+    return ~narrow(sh, [&](auto&& f) { each([&](uint32_t at) { f(~at, one_each); }); }, ~vocab, 0xffffffffu, 0, (u64)ties + 1, &ignored);
+}
+
 // ---------------------------------------------------------------- the draw from a list
-// `listed` <= LIST_MAX scores and their rows in sh.list_*, in row order, among them all that remain.
+// `listed` <= LIST_MAX scores and their rows in sh.list_*, in any order, among them all that remain.
 __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& a, int64_t row, const Settings& set, const FixedExp& weigh, int listed) {
     const int tid = threadIdx.x;
     const u64 least_w = set.least_weight(a.shift);
-    u64 w[LIST_ITEMS];
-#pragma unroll
-    for (int q = 0; q < LIST_ITEMS; ++q) w[q] = q * SAMPLE_NT + tid < listed ? weigh(sh.list_z[q * SAMPLE_NT + tid]) : 0;
-    if (listed <= 256) {
-        // every item's rank and the weights before it, by comparing all pairs
+    if (listed <= PAIRS) {
+        // every item's rank, the weights ranked before it, and, once it is known what remains, those of lower rows: by
+        // comparing all pairs, the block's threads in slices of the list
         int log_width = 6;
         while ((1 << log_width) < listed) ++log_width;
-        const int i = tid & ((1 << log_width) - 1);
-        if (tid < 256) { sh.rank[tid] = 0; sh.before[tid] = 0; }
+        const int i = tid & ((1 << log_width) - 1), slice = tid >> log_width, slices = SAMPLE_NT >> log_width;
+        const float zi = i < listed ? sh.list_z[i] : 0.0f;
+        const uint32_t at = i < listed ? sh.list_at[i] : 0;
+        u64 w = 0;
+        if (tid < listed) w = weigh.directly(zi);
+        if (tid < PAIRS) { sh.pair_rank[tid] = 0; sh.pair_sum[tid] = 0; sh.pair_w[tid] = w; }
         __syncthreads();
         if (i < listed) {
-            const float zi = sh.list_z[i];
             uint32_t rank = 0;
             u64 before = 0;
-            for (int j = tid >> log_width; j < listed; j += SAMPLE_NT >> log_width) {
+            for (int j = slice; j < listed; j += slices) {
                 const float zj = sh.list_z[j];
-                if (zj > zi || (zj == zi && j < i)) {
+                if (zj > zi || (zj == zi && sh.list_at[j] < at)) {
                     ++rank;
-                    if (set.by_mass()) before += weigh(zj);
+                    before += sh.pair_w[j];
                 }
             }
             if (rank) {
-                atomicAdd(&sh.rank[i], rank);
-                if (set.by_mass()) atomicAdd(&sh.before[i], before);
+                atomicAdd(&sh.pair_rank[i], rank);
+                atomicAdd(&sh.pair_sum[i], before);
             }
         }
         __syncthreads();
-        if (set.by_count() && tid < listed && sh.rank[tid] >= (uint32_t)set.top_k) w[0] = 0;
+        if (set.by_count() && tid < listed && sh.pair_rank[tid] >= (uint32_t)set.top_k) w = 0;
         if (set.by_mass()) {
-            const double target = (double)block_total(sh, w[0]) * (double)set.top_p;
-            if (tid < listed && sh.rank[tid] > 0 && !((double)sh.before[tid] < target)) w[0] = 0;
+            const double target = (double)block_total(sh, w) * (double)set.top_p;
+            if (tid < listed && sh.pair_rank[tid] > 0 && !((double)sh.pair_sum[tid] < target)) w = 0;
         }
-    } else {
-        float cut = -INFINITY;
-        int64_t ties = INT64_MAX;
-        const uint32_t top = pattern((float)weigh.best);
-        if (set.by_count() && set.top_k < listed) {
-            u64 above;
-            cut = score_of(narrow(sh, [&](auto&& f) {
-                for (int i = tid; i < listed; i += SAMPLE_NT) f(pattern(sh.list_z[i]), one_each);
-            }, 1u, top, 0, (u64)set.top_k, &above));
-            ties = set.top_k - (int64_t)above;
+        if (w < least_w) w = 0;
+        __syncthreads();
+        if (tid < PAIRS) { sh.pair_w[tid] = w; sh.pair_sum[tid] = 0; }
+        const u64 all = block_total(sh, w), least = set.goal(all);
+        if (i < listed) {
+            u64 before = 0;
+            for (int j = slice; j < listed; j += slices)
+                if (sh.list_at[j] < at) before += sh.pair_w[j];
+            if (before) atomicAdd(&sh.pair_sum[i], before);
         }
-        if (set.by_mass()) {
-            u64 sum = 0;
-#pragma unroll
-            for (int q = 0; q < LIST_ITEMS; ++q)
-                if (w[q] && sh.list_z[q * SAMPLE_NT + tid] > cut) sum += w[q];
-            const u64 over = block_total(sh, sum), w_cut = ties < INT64_MAX ? weigh(cut) : 0;
-            const double target = (double)(over + w_cut * (u64)(ties < INT64_MAX ? ties : 0)) * (double)set.top_p;
-            const u64 least = max((u64)ceil(target), (u64)1);
-            if (over >= least) {
-                u64 above;
-                const float floor_z = cut;
-                cut = score_of(narrow(sh, [&](auto&& f) {
-                    for (int i = tid; i < listed; i += SAMPLE_NT) {
-                        const float z = sh.list_z[i];
-                        if (z > floor_z) f(pattern(z), [&] { return weigh(z); });
-                    }
-                }, 1u, top, 0, least, &above));
-                ties = ties_within(target, above, weigh(cut));
-            } else if (w_cut) {
-                ties = min(ties, ties_within(target, over, w_cut));
-            }
-        }
-        u64 run = 0;
-#pragma unroll
-        for (int q = 0; q < LIST_ITEMS; ++q) {
-            const int i = q * SAMPLE_NT + tid;
-            const bool at_cut = i < listed && sh.list_z[i] == cut;
-            u64 total;
-            const u64 before = run + block_scan(sh, at_cut ? 1 : 0, &total);
-            run += total;
-            if (i >= listed || sh.list_z[i] < cut || (at_cut && (int64_t)before >= ties)) w[q] = 0;
-        }
+        __syncthreads();
+        if (tid < listed && w && sh.pair_sum[tid] < least && sh.pair_sum[tid] + w >= least) write_draw(a, row, at, w, all);
+        return;
     }
-    u64 before[LIST_ITEMS], all = 0;
+    make_table(sh.table, tid, SAMPLE_NT);
+    __syncthreads();
+    u64 w[LIST_ITEMS];
+    float z[LIST_ITEMS];
+    uint32_t at[LIST_ITEMS];
 #pragma unroll
     for (int q = 0; q < LIST_ITEMS; ++q) {
-        if (w[q] < least_w) w[q] = 0;
-        before[q] = 0;
-        if (q * SAMPLE_NT >= listed) continue;
-        u64 total;
-        before[q] = all + block_scan(sh, w[q], &total);
-        all += total;
+        const int i = q * SAMPLE_NT + tid;
+        z[q] = i < listed ? sh.list_z[i] : -INFINITY;
+        at[q] = i < listed ? sh.list_at[i] : 0;
+        w[q] = weigh(z[q]);
     }
-    const u64 least = set.goal(all);
+    float cut = -INFINITY;
+    int64_t ties = INT64_MAX;
+    float lowest = INFINITY, best = -INFINITY;
+#pragma unroll
+    for (int q = 0; q < LIST_ITEMS; ++q) {
+        best = fmaxf(best, z[q]);
+        if (z[q] > -INFINITY) lowest = fminf(lowest, z[q]);
+    }
+    block_range(sh, lowest, best);
+    const uint32_t bottom = pattern(lowest), top = pattern(best);
+    if (set.by_count() && set.top_k < listed) {
+        u64 above;
+        cut = score_of(narrow(sh, [&](auto&& f) {
+#pragma unroll
+            for (int q = 0; q < LIST_ITEMS; ++q) f(pattern(z[q]), one_each);
+        }, bottom, top, 0, (u64)set.top_k, &above));
+        ties = set.top_k - (int64_t)above;
+    }
+    if (set.by_mass()) {
+        u64 sum = 0;
+#pragma unroll
+        for (int q = 0; q < LIST_ITEMS; ++q) sum += z[q] > cut ? w[q] : 0;
+        const u64 over = block_total(sh, sum), w_cut = ties < INT64_MAX ? weigh(cut) : 0;
+        const double target = (double)(over + w_cut * (u64)(ties < INT64_MAX ? ties : 0)) * (double)set.top_p;
+        const u64 least = max((u64)ceil(target), (u64)1);
+        if (over >= least) {
+            u64 above;
+            const float floor_z = cut;
+            cut = score_of(narrow(sh, [&](auto&& f) {
+#pragma unroll
+                for (int q = 0; q < LIST_ITEMS; ++q)
+                    if (z[q] > floor_z) f(pattern(z[q]), [&] { return w[q]; });
+            }, bottom, top, 0, least, &above));
+            ties = ties_within(target, above, weigh(cut));
+        } else if (w_cut) {
+            ties = min(ties, ties_within(target, over, w_cut));
+        }
+    }
+    const uint32_t tie_end = first_tie_out(sh, [&](auto&& f) {
+#pragma unroll
+        for (int q = 0; q < LIST_ITEMS; ++q)
+            if (z[q] == cut) f(at[q]);
+    }, ties, (uint32_t)a.vocab);
+    u64 sum = 0;
+#pragma unroll
+    for (int q = 0; q < LIST_ITEMS; ++q) {
+        if (!(z[q] > cut || (z[q] == cut && at[q] < tie_end)) || w[q] < least_w) w[q] = 0;
+        sum += w[q];
+    }
+    const u64 all = block_total(sh, sum);
+    u64 before;
+    // the row, from the first, at which the running sum reaches the goal
+    const uint32_t drawn = ~narrow(sh, [&](auto&& f) {
+#pragma unroll
+        for (int q = 0; q < LIST_ITEMS; ++q)
+            if (w[q]) f(~at[q], [&] { return w[q]; });
+    }, ~(uint32_t)a.vocab, 0xffffffffu, 0, set.goal(all), &before);
 #pragma unroll
     for (int q = 0; q < LIST_ITEMS; ++q)
-        if (w[q] && before[q] < least && before[q] + w[q] >= least) write_draw(a, row, sh.list_at[q * SAMPLE_NT + tid], w[q], all);
+        if (w[q] && at[q] == drawn) write_draw(a, row, drawn, w[q], all);
 }
 
 // ---------------------------------------------------------------- a row by one block
@@ -470,56 +587,35 @@ template <class T> struct RowPasses {
             if (hold(from, to)) f(from, g);
         }
     }
-    // The scores at or above thr to the list, in row order; -> their number, nothing written where that exceeds LIST_MAX.
+    // The scores at or above thr to the list; -> their number, of which the list holds LIST_MAX.
     __device__ __forceinline__ int compact(SampleShared& sh, float thr) const {
-        auto count = [&](const Piece<T>& v) {
-            uint32_t c = 0;
+        __syncthreads();
+        if (tid == 0) sh.listed = 0;
+        __syncthreads();
+        pieces(0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; }, [&](int, int at, const Piece<T>& v) {
+            float top = v.get(0);
 #pragma unroll
-            for (int e = 0; e < N; ++e) c += v.get(e) >= thr ? 1 : 0;
-            return c;
-        };
-        const u64 total = sum_parts(sh, [&](const Piece<T>& v, int) { return (u64)count(v); });
-        if (total > LIST_MAX) return LIST_MAX + 1;
-        parts_that(sh, total, [](u64 from, u64 to) { return from < to; }, [&](u64 before, int g) {
-            uint32_t from = (uint32_t)before;
-            in_order(g * per_group, min((g + 1) * per_group, steps), [&](int, int at, const Piece<T>& v) {
-                const uint32_t c = count(v);
-                const u64 inc = wave_scan(c);
-                uint32_t to = from + (uint32_t)inc - c;
+            for (int e = 1; e < N; ++e) top = fmaxf(top, v.get(e));
+            if (!__ballot(top >= thr)) return;
 #pragma unroll
-                for (int e = 0; e < N; ++e) {
-                    const float z = v.get(e);
-                    if (z >= thr) {
-                        sh.list_z[to] = z;
-                        sh.list_at[to] = (uint32_t)(at + e);
-                        ++to;
-                    }
-                }
-                from += (uint32_t)last_lane(inc);
-            });
+            for (int e = 0; e < N; ++e) append(sh, v.get(e) >= thr, v.get(e), (uint32_t)(at + e));
         });
         __syncthreads();
-        return (int)total;
+        return (int)sh.listed;
     }
 };
 
 template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared& sh, const T* scores, const SampleArgs& a, int64_t row) {
     constexpr int N = Piece<T>::N;
     RowPasses<T> pass(Source<T>(scores, a, row));
-    const int tid = threadIdx.x, lane = pass.lane;
+    const int tid = threadIdx.x;
     const Settings set(a, row);
-    make_table(sh.table, tid, SAMPLE_NT);
     // ---- the largest score of each thread, and of the row
     float mine = -INFINITY;
     pass.each([&](float z) { mine = fmaxf(mine, z); });
-    float best = mine;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
-    __syncthreads();
-    if (lane == 0) sh.red[pass.wave] = __float_as_uint(best);
+    float best = mine, lowest = mine > -INFINITY ? mine : INFINITY;
     if (tid == 0) sh.first = 0xffffffffu;
-    __syncthreads();
-    for (int w = 0; w < SAMPLE_WAVES; ++w) best = fmaxf(best, __uint_as_float((uint32_t)sh.red[w]));
+    block_range(sh, lowest, best);
     if (best == -INFINITY) {
         if (tid == 0) write_certain(a, row, -1);
         return;
@@ -544,7 +640,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
     if (best == INFINITY) {
         pass.src.infinite = true;
         mine = mine == INFINITY ? 0.0f : -INFINITY;
-        best = 0.0f;
+        best = lowest = 0.0f;
     }
     const FixedExp weigh(best, set.tau, a.shift, sh.table);
     const u64 least_w = set.least_weight(a.shift);
@@ -552,9 +648,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
     // ---- few rows can remain: a list of them
     float thr = -INFINITY;
     if (set.by_count() && set.top_k <= SAMPLE_NT) {
-        u64 above;
-        const uint32_t o = narrow(sh, [&](auto&& f) { f(pattern(mine), one_each); }, 1u, pattern(best), 0, (u64)set.top_k, &above, 2);
-        thr = o > 0x00800000u ? score_of(o) : LOWEST;            // fewer than top_k threads hold anything: everything
+        thr = bound_of(sh, [&](auto&& f) { f(pattern(mine), one_each); }, lowest, best, set.top_k);
     } else if (!set.by_count() && !set.by_mass() && least_w) {
         thr = set.min_p_bound(best);
     }
@@ -562,6 +656,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
         const int listed = pass.compact(sh, thr);
         if (listed <= LIST_MAX) return draw_listed(sh, a, row, set, weigh, listed);
     }
+    make_table(sh.table, tid, SAMPLE_NT);                        // the next barrier is clear_bins' or sum_parts'
 
     // ---- the lowest score that remains (cut), and how many of the rows at it
     float cut = -INFINITY;
@@ -789,16 +884,15 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kern
     const float* group_max = work.group_max + row * work.groups;
     // a contiguous run of groups a thread
     const int per = (work.groups + SAMPLE_NT - 1) / SAMPLE_NT, g0 = min(tid * per, work.groups), g1 = min(g0 + per, work.groups);
-    float best = -INFINITY;
-    for (int g = g0; g < g1; ++g) best = fmaxf(best, group_max[g]);
+    float best = -INFINITY, lowest = INFINITY;
+    for (int g = g0; g < g1; ++g) {
+        const float m = group_max[g];
+        best = fmaxf(best, m);
+        if (m > -INFINITY) lowest = fminf(lowest, m);
+    }
     const float mine = best;
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) best = fmaxf(best, __shfl_xor(best, o));
-    if (lane == 0) sh.red[wave] = __float_as_uint(best);
-    if (tid == 0) sh.first = 0xffffffffu;
-    make_table(sh.table, tid, SAMPLE_NT);
-    __syncthreads();
-    for (int v = 0; v < SAMPLE_WAVES; ++v) best = fmaxf(best, __uint_as_float((uint32_t)sh.red[v]));
+    if (tid == 0) { sh.first = 0xffffffffu; sh.listed = sh.found = 0; }
+    block_range(sh, lowest, best);
     if (best == -INFINITY) {
         if (tid == 0) write_certain(a, row, -1);
         return;
@@ -822,53 +916,40 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kern
     int mode = best == INFINITY ? ROW_WHOLE : set.by_count() ? ROW_WHOLE : set.by_mass() ? ROW_MASS : ROW_SUM;
     if (best < INFINITY) {
         if (set.by_count() && set.top_k <= SAMPLE_NT) {
-            u64 above;
-            const uint32_t o = narrow(sh, [&](auto&& f) {
+            thr = bound_of(sh, [&](auto&& f) {
                 for (int g = g0; g < g1; ++g) f(pattern(group_max[g]), one_each);
-            }, 1u, pattern(best), 0, (u64)set.top_k, &above, 2);
-            thr = o > 0x00800000u ? score_of(o) : LOWEST;            // fewer than top_k groups hold anything: everything
+            }, lowest, best, set.top_k);
         } else if (!set.by_count() && !set.by_mass() && set.min_p > 0.0f) {
             thr = set.min_p_bound(best);
         }
     }
     if (thr > -INFINITY) {
-        // the groups that reach the bound, in order, where the list's rows go later
-        uint32_t count = 0;
-        for (int g = g0; g < g1; ++g) count += group_max[g] >= thr ? 1 : 0;
-        u64 found;
-        uint32_t to = (uint32_t)block_scan(sh, count, &found);
+        // the groups that reach the bound, and their scores that do
+        uint32_t* group = (uint32_t*)sh.bin;
+        __syncthreads();
+        if (tid == 0) sh.found = 0;
+        __syncthreads();
+        for (int g = g0; g < g1; ++g)
+            if (group_max[g] >= thr) {
+                const uint32_t i = atomicAdd(&sh.found, 1u);
+                if (i < LIST_MAX) group[i] = (uint32_t)g;
+            }
+        __syncthreads();
+        const int found = (int)sh.found;
         if (found <= LIST_MAX) {
-            uint32_t* group = (uint32_t*)sh.bin;
-            for (int g = g0; g < g1; ++g)
-                if (group_max[g] >= thr) group[to++] = (uint32_t)g;
+            // 64 scores a wave, two groups, two such at a time
+            for (int c = 2 * wave; 2 * c < found; c += 2 * SAMPLE_WAVES) {
+                const int k0 = 2 * c + (lane >> 5), k1 = k0 + 2;
+                const int at0 = k0 < found ? (int)group[k0] * GROUP + (lane & (GROUP - 1)) : src.vocab;
+                const int at1 = k1 < found ? (int)group[k1] * GROUP + (lane & (GROUP - 1)) : src.vocab;
+                const float z0 = src.one(at0), z1 = src.one(at1);
+                append(sh, z0 >= thr, z0, (uint32_t)at0);
+                append(sh, z1 >= thr, z1, (uint32_t)at1);
+            }
             __syncthreads();
-            // 64 scores a wave: two groups
-            const int chunks = ((int)found + 1) / 2;
-            auto score = [&](int c, int* at) {
-                const int k = 2 * c + (lane >> 5);
-                *at = k < (int)found ? (int)group[k] * GROUP + (lane & (GROUP - 1)) : src.vocab;
-                return src.one(*at);
-            };
-            for (int c = wave; c < chunks; c += SAMPLE_WAVES) {
-                int at;
-                const unsigned long long m = __ballot(score(c, &at) >= thr);
-                if (lane == 0) sh.part[c] = (u64)__popcll(m);
-            }
-            const u64 listed = scan_parts(sh, chunks);
-            if (listed <= LIST_MAX) {
-                for (int c = wave; c < chunks; c += SAMPLE_WAVES) {
-                    int at;
-                    const float z = score(c, &at);
-                    const unsigned long long m = __ballot(z >= thr);
-                    if (z >= thr) {
-                        const uint32_t i = (uint32_t)sh.part[c] + (uint32_t)__popcll(m & ((1ull << lane) - 1));
-                        sh.list_z[i] = z;
-                        sh.list_at[i] = (uint32_t)at;
-                    }
-                }
-                __syncthreads();
-                return draw_listed(sh, a, row, set, weigh, (int)listed);
-            }
+            const int listed = (int)sh.listed;
+            __syncthreads();
+            if (listed <= LIST_MAX) return draw_listed(sh, a, row, set, weigh, listed);
         }
     }
     if (tid == 0) {
@@ -1072,16 +1153,10 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_rest_kern
         }
     }, pattern(lo), pattern(hi), state.above, state.least, &above));
     const int64_t ties = ties_within(state.target, above, weigh(cut));
-    u64 at_cut = 0;
-    for (int i = tid; i < members; i += SAMPLE_NT) at_cut += sh.list_z[i] == cut ? 1 : 0;
-    uint32_t tie_end = 0xffffffffu;              // rows at the cut from this one on are out
-    if ((int64_t)block_total(sh, at_cut) > ties) {
-        u64 ignored;
-        tie_end = ~narrow(sh, [&](auto&& f) {
-            for (int i = tid; i < members; i += SAMPLE_NT)
-                if (sh.list_z[i] == cut) f(~sh.list_at[i], one_each);
-        }, ~(uint32_t)a.vocab, 0xffffffffu, 0, (u64)ties + 1, &ignored);
-    }
+    const uint32_t tie_end = first_tie_out(sh, [&](auto&& f) {
+        for (int i = tid; i < members; i += SAMPLE_NT)
+            if (sh.list_z[i] == cut) f(sh.list_at[i]);
+    }, ties, (uint32_t)a.vocab);
     auto weight_at = [&](float z, uint32_t at) {
         const u64 w = weigh(z);
         return (z > cut || (z == cut && at < tie_end)) && w >= least_w ? w : (u64)0;
