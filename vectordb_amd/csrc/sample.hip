@@ -144,7 +144,7 @@ struct FixedExp {
     }
     __device__ __forceinline__ int bin(float z) const {              // distance from the best in steps of 1/32 of a power of two
         const int k = (int)(uint32_t)__double_as_longlong(fma((double)z - best, c, NEAREST));
-        return min((-k) >> 5, BINS - 1);
+        return (int)min((uint32_t)(-k) >> 5, (uint32_t)(BINS - 1));
     }
     // the same without the table, for a few scores: exp2() to the last bits of a double
     __device__ __forceinline__ u64 directly(float z) const {
@@ -201,6 +201,7 @@ __device__ __forceinline__ u64 last_lane(u64 v) {
     return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
 }
 __device__ __forceinline__ u64 wave_sum(u64 v) { return last_lane(wave_scan(v)); }
+// (the loops over the waves' sums are unrolled: their loads go out together)
 // exclusive prefix of v over the block; *total = its sum
 __device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -209,6 +210,7 @@ __device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* total) {
     if (lane == 63) sh.red[wave] = inc;
     __syncthreads();
     u64 all = 0, base = 0;
+#pragma unroll
     for (int w = 0; w < SAMPLE_WAVES; ++w) {
         if (w < wave) base += sh.red[w];
         all += sh.red[w];
@@ -222,6 +224,7 @@ __device__ __forceinline__ u64 block_total(SampleShared& sh, u64 v) {
     if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
+#pragma unroll
     for (int w = 0; w < SAMPLE_WAVES; ++w) v += sh.red[w];
     return v;
 }
@@ -241,9 +244,21 @@ __device__ __forceinline__ void clear_bins(SampleShared& sh) {
     sh.bin[threadIdx.x + SAMPLE_NT] = 0;
     __syncthreads();
 }
-__device__ __forceinline__ void make_table(double* table, int tid, int nt) {
-    for (int j = tid; j < EXP_STEPS; j += nt) table[j] = exp2((double)j / EXP_STEPS);
-}
+// 2^(j / 1024), by exp's series to the last bits of a double
+struct ExpTable {
+    double v[EXP_STEPS];
+    constexpr ExpTable() : v() {
+        for (int j = 0; j < EXP_STEPS; ++j) {
+            const double x = 0.69314718055994530942 * j / EXP_STEPS;
+            double sum = 1.0;
+            for (int k = 20; k >= 1; --k) sum = 1.0 + sum * x / k;
+            v[j] = sum;
+        }
+    }
+};
+__device__ constexpr ExpTable EXP_TABLE{};
+static_assert(EXP_STEPS == SAMPLE_NT, "a thread an entry");
+__device__ __forceinline__ void make_table(double* table) { table[threadIdx.x] = EXP_TABLE.v[threadIdx.x]; }
 // the first bin, from the top or from the bottom, at which the running sum, from `above`, reaches target: sh.found its
 // number in that order (BINS: none), sh.found_sum the sum before it
 __device__ static void find_bin(SampleShared& sh, u64 above, u64 target, bool from_top) {
@@ -354,6 +369,7 @@ __device__ __forceinline__ void block_range(SampleShared& sh, float& lowest, flo
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = ((u64)__float_as_uint(lowest) << 32) | __float_as_uint(best);
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < SAMPLE_WAVES; ++w) {
         best = fmaxf(best, __uint_as_float((uint32_t)sh.red[w]));
         lowest = fminf(lowest, __uint_as_float((uint32_t)(sh.red[w] >> 32)));
@@ -434,7 +450,7 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
         if (tid < listed && w && sh.pair_sum[tid] < least && sh.pair_sum[tid] + w >= least) write_draw(a, row, at, w, all);
         return;
     }
-    make_table(sh.table, tid, SAMPLE_NT);
+    make_table(sh.table);
     __syncthreads();
     u64 w[LIST_ITEMS];
     float z[LIST_ITEMS];
@@ -509,6 +525,40 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
 }
 
 // ---------------------------------------------------------------- a row by one block
+// Pieces of a loop, AHEAD loads in flight while the ones before are worked on: f(step, first element, piece) for steps
+// [from, to), `at(step)` the first element of this lane's piece; `prologue` runs while the first loads are under way.  A step is
+// kept apart from the next (sched_barrier): the compiler would interleave them and run out of registers.
+template <class T, class At, class F, class P>
+__device__ __forceinline__ void stream_pieces(const Source<T>& src, int from, int to, At&& at, F&& f, P&& prologue) {
+    Piece<T> next[AHEAD];
+    uint32_t bits[AHEAD];
+    auto fetch = [&](int t0) {
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            const int i = t0 + j < to ? at(t0 + j) : src.vocab;
+            next[j] = src.load(i);
+            bits[j] = src.bits(i);
+        }
+    };
+    fetch(from);
+    prologue();
+#pragma unroll 1
+    for (int t0 = from; t0 < to; t0 += AHEAD) {
+        Piece<T> now[AHEAD];
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            now[j] = next[j];
+            src.finish(now[j], bits[j]);
+        }
+        if (t0 + AHEAD < to) fetch(t0 + AHEAD);
+#pragma unroll
+        for (int j = 0; j < AHEAD; ++j) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (t0 + j < to) f(t0 + j, at(t0 + j), now[j]);
+        }
+    }
+}
+
 template <class T> struct RowPasses {
     static constexpr int N = Piece<T>::N;
     Source<T> src;
@@ -523,47 +573,17 @@ template <class T> struct RowPasses {
         parts = SAMPLE_WAVES * groups;
         share = steps * 64 * N;
     }
-    // Pieces of a loop, AHEAD loads in flight while the ones before are worked on: f(step, first element, piece) for steps
-    // [from, to), `at(step)` the first element of this lane's piece.  A step is kept apart from the next (sched_barrier): the
-    // compiler would interleave them and run out of registers.
-    template <class At, class F> __device__ __forceinline__ void pieces(int from, int to, At&& at, F&& f) const {
-        Piece<T> next[AHEAD];
-        uint32_t bits[AHEAD];
-        auto fetch = [&](int t0) {
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                const int i = t0 + j < to ? at(t0 + j) : src.vocab;
-                next[j] = src.load(i);
-                bits[j] = src.bits(i);
-            }
-        };
-        fetch(from);
-#pragma unroll 1
-        for (int t0 = from; t0 < to; t0 += AHEAD) {
-            Piece<T> now[AHEAD];
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                now[j] = next[j];
-                src.finish(now[j], bits[j]);
-            }
-            fetch(t0 + AHEAD);
-#pragma unroll
-            for (int j = 0; j < AHEAD; ++j) {
-                __builtin_amdgcn_sched_barrier(0);
-                if (t0 + j < to) f(t0 + j, at(t0 + j), now[j]);
-            }
-        }
-    }
     // every score, in no order: f(z)
     template <class F> __device__ __forceinline__ void each(F&& f) const {
-        pieces(0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; }, [&](int, int, const Piece<T>& v) {
+        stream_pieces(src, 0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; },
+                      [&](int, int, const Piece<T>& v) {
 #pragma unroll
-            for (int e = 0; e < N; ++e) f(v.get(e));
-        });
+                          for (int e = 0; e < N; ++e) f(v.get(e));
+                      }, [] {});
     }
     // the steps [from, to) of the wave's share, in order: f(step, first element, piece)
     template <class F> __device__ __forceinline__ void in_order(int from, int to, F&& f) const {
-        pieces(from, to, [&](int t) { return wave * share + (t * 64 + lane) * N; }, f);
+        stream_pieces(src, from, to, [&](int t) { return wave * share + (t * 64 + lane) * N; }, f, [] {});
     }
     // sh.part = the running sums of value(piece, first element) before each part; -> their sum
     template <class Value> __device__ __forceinline__ u64 sum_parts(SampleShared& sh, Value&& value) const {
@@ -592,14 +612,15 @@ template <class T> struct RowPasses {
         __syncthreads();
         if (tid == 0) sh.listed = 0;
         __syncthreads();
-        pieces(0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; }, [&](int, int at, const Piece<T>& v) {
-            float top = v.get(0);
+        stream_pieces(src, 0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; },
+                      [&](int, int at, const Piece<T>& v) {
+                          float top = v.get(0);
 #pragma unroll
-            for (int e = 1; e < N; ++e) top = fmaxf(top, v.get(e));
-            if (!__ballot(top >= thr)) return;
+                          for (int e = 1; e < N; ++e) top = fmaxf(top, v.get(e));
+                          if (!__ballot(top >= thr)) return;
 #pragma unroll
-            for (int e = 0; e < N; ++e) append(sh, v.get(e) >= thr, v.get(e), (uint32_t)(at + e));
-        });
+                          for (int e = 0; e < N; ++e) append(sh, v.get(e) >= thr, v.get(e), (uint32_t)(at + e));
+                      }, [] {});
         __syncthreads();
         return (int)sh.listed;
     }
@@ -656,7 +677,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
         const int listed = pass.compact(sh, thr);
         if (listed <= LIST_MAX) return draw_listed(sh, a, row, set, weigh, listed);
     }
-    make_table(sh.table, tid, SAMPLE_NT);                        // the next barrier is clear_bins' or sum_parts'
+    make_table(sh.table);                        // the next barrier is clear_bins' or sum_parts'
 
     // ---- the lowest score that remains (cut), and how many of the rows at it
     float cut = -INFINITY;
@@ -807,7 +828,7 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_kernel(co
 // 6 sample_rest (a block per row): the border among the members and the draw; rows for which a list was too short go through
 //   all passes by one block
 static constexpr int GROUP = 32, STREAM_NT = 256, STREAM_PIECES = 4;
-enum RowMode { ROW_DONE = 0, ROW_WHOLE = 1, ROW_SUM = 2, ROW_MASS = 3 };
+enum RowMode { ROW_DONE = 0, ROW_WHOLE = 1, ROW_SUM = 2, ROW_MASS = 3, ROW_LIST = 4 };
 struct RowState {
     u64 above, least;                // weights above the bin of the border; the running sum that the border reaches
     double target;
@@ -816,12 +837,13 @@ struct RowState {
     uint32_t members;
 };
 static constexpr int PARTS = SAMPLE_WAVES * GROUPS;                 // at most, per row
+static constexpr int PARTS_EACH = 4 * (STREAM_NT / 64);             // parts of a streaming block: four a wave
 struct SampleWork {
     float* group_max; int groups;    // [n][groups]
     RowState* state;                 // [n]
     u64* hist;                       // [n][BINS]
-    u64* part; int parts, part_len;  // [n][PARTS], scores of a part (a multiple of 512)
-    float* member_z; uint32_t* member_at;                           // [n][LIST_MAX]
+    u64* part; int parts, part_len;    // [n][PARTS], scores of a part (a multiple of 512)
+    float* member_z; uint32_t* member_at;           // [n][LIST_MAX]
     int64_t bytes;
 };
 static SampleWork sample_work(void* base, int64_t n, int64_t vocab) {
@@ -843,6 +865,13 @@ static SampleWork sample_work(void* base, int64_t n, int64_t vocab) {
     w.member_at = (uint32_t*)take(n * LIST_MAX * 4);
     w.bytes = at - (char*)base;
     return w;
+}
+// What a row's settings make of it, before its scores are seen.  Min-p alone mostly leaves few rows where it is 1/64 or more.
+__host__ __device__ static inline RowMode mode_of(float tau, int top_k, float top_p, float min_p) {
+    if (!(tau > 0.0f) || top_k == 1 || top_p <= 0.0f) return ROW_LIST;
+    if (top_k > 1) return top_k <= SAMPLE_NT ? ROW_LIST : ROW_WHOLE;
+    if (top_p < 1.0f) return ROW_MASS;
+    return min_p >= 0.015625f ? ROW_LIST : ROW_SUM;
 }
 
 template <class T>
@@ -875,21 +904,35 @@ __global__ void __launch_bounds__(STREAM_NT) sample_groups_kernel(const T* __res
     }
 }
 
-template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
-    __shared__ SampleShared sh;
-    const int64_t row = blockIdx.x;
+// the smallest and the largest of a row's group maxima; a contiguous run [g0, g1) of groups a thread
+struct GroupRun {
+    const float* max;
+    int g0, g1;
+    __device__ __forceinline__ GroupRun(const SampleWork& work, int64_t row) : max(work.group_max + row * work.groups) {
+        const int per = (work.groups + SAMPLE_NT - 1) / SAMPLE_NT;
+        g0 = min((int)threadIdx.x * per, work.groups);
+        g1 = min(g0 + per, work.groups);
+    }
+    __device__ __forceinline__ void range(float& lowest, float& best) const {
+        best = -INFINITY;
+        lowest = INFINITY;
+        for (int g = g0; g < g1; ++g) {
+            const float m = max[g];
+            best = fmaxf(best, m);
+            if (m > -INFINITY) lowest = fminf(lowest, m);
+        }
+    }
+};
+
+template <class T> __device__ __forceinline__ void sample_pick(SampleShared& sh, const T* scores, const SampleArgs& a, const SampleWork& work, int64_t row) {
     const Source<T> src(scores, a, row);
     const Settings set(a, row);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const float* group_max = work.group_max + row * work.groups;
-    // a contiguous run of groups a thread
-    const int per = (work.groups + SAMPLE_NT - 1) / SAMPLE_NT, g0 = min(tid * per, work.groups), g1 = min(g0 + per, work.groups);
-    float best = -INFINITY, lowest = INFINITY;
-    for (int g = g0; g < g1; ++g) {
-        const float m = group_max[g];
-        best = fmaxf(best, m);
-        if (m > -INFINITY) lowest = fminf(lowest, m);
-    }
+    const GroupRun groups(work, row);
+    const float* group_max = groups.max;
+    const int g0 = groups.g0, g1 = groups.g1;
+    float best, lowest;
+    groups.range(lowest, best);
     const float mine = best;
     if (tid == 0) { sh.first = 0xffffffffu; sh.listed = sh.found = 0; }
     block_range(sh, lowest, best);
@@ -911,19 +954,12 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kern
         }
         return;
     }
-    const FixedExp weigh(best, set.tau, a.shift, sh.table);
-    float thr = -INFINITY;
-    int mode = best == INFINITY ? ROW_WHOLE : set.by_count() ? ROW_WHOLE : set.by_mass() ? ROW_MASS : ROW_SUM;
-    if (best < INFINITY) {
-        if (set.by_count() && set.top_k <= SAMPLE_NT) {
-            thr = bound_of(sh, [&](auto&& f) {
-                for (int g = g0; g < g1; ++g) f(pattern(group_max[g]), one_each);
-            }, lowest, best, set.top_k);
-        } else if (!set.by_count() && !set.by_mass() && set.min_p > 0.0f) {
-            thr = set.min_p_bound(best);
-        }
-    }
-    if (thr > -INFINITY) {
+    const int mode = best == INFINITY ? ROW_WHOLE : mode_of(set.tau, set.top_k, set.top_p, set.min_p);
+    if (mode == ROW_LIST) {
+        const FixedExp weigh(best, set.tau, a.shift, sh.table);
+        const float thr = !set.by_count() ? set.min_p_bound(best) : bound_of(sh, [&](auto&& f) {
+            for (int g = g0; g < g1; ++g) f(pattern(group_max[g]), one_each);
+        }, lowest, best, set.top_k);
         // the groups that reach the bound, and their scores that do
         uint32_t* group = (uint32_t*)sh.bin;
         __syncthreads();
@@ -954,68 +990,142 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kern
     }
     if (tid == 0) {
         work.state[row].best = best;
-        work.state[row].mode = mode;
+        work.state[row].mode = mode == ROW_LIST ? ROW_WHOLE : mode;
     }
 }
 
-// Parts [p0, p0 + count) of a row, one wave each after the other: f(piece, first element) is added up into work.part.
-template <class T, class F>
-__device__ __forceinline__ void stream_parts(const Source<T>& src, const SampleWork& work, int64_t row, int p0, int count, F&& f) {
-    constexpr int N = Piece<T>::N;
+// Parts [p0, p0 + PARTS_EACH) of a row, a run of them a wave: out[part] = the sum of f(piece, first element)
+template <class T, class F, class P>
+__device__ __forceinline__ void stream_parts(const Source<T>& src, const SampleWork& work, int p0, u64* out, F&& f, P&& prologue) {
+    constexpr int N = Piece<T>::N, EACH = PARTS_EACH / (STREAM_NT / 64);
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    for (int p = p0 + wave; p < min(p0 + count, work.parts); p += STREAM_NT / 64) {
-        u64 sum = 0;
-        const int end = (p + 1) * work.part_len;
-        for (int at0 = p * work.part_len; at0 < end; at0 += 512) {
-            Piece<T> x[512 / (64 * N)];
-            uint32_t bits[512 / (64 * N)];
+    const int first = p0 + EACH * wave, end = min(first + EACH, work.parts), steps = work.part_len / (64 * N);
+    u64 sum = 0;
+    stream_pieces(src, 0, max(end - first, 0) * steps, [&](int t) { return first * work.part_len + (t * 64 + lane) * N; },
+                  [&](int t, int at, const Piece<T>& v) {
+                      sum += f(v, at);
+                      if ((t + 1) % steps) return;
+                      sum = wave_sum(sum);
+                      if (lane == 0) out[first + t / steps] = sum;
+                      sum = 0;
+                  }, prologue);
+}
+__device__ __forceinline__ void stream_table(double* table) {
 #pragma unroll
-            for (int j = 0; j < 512 / (64 * N); ++j) {
-                x[j] = src.load(at0 + (j * 64 + lane) * N);
-                bits[j] = src.bits(at0 + (j * 64 + lane) * N);
-            }
-#pragma unroll
-            for (int j = 0; j < 512 / (64 * N); ++j) {
-                src.finish(x[j], bits[j]);
-                sum += f(x[j], at0 + (j * 64 + lane) * N);
-            }
-        }
-        sum = wave_sum(sum);
-        if (lane == 0) work.part[row * PARTS + p] = sum;
-    }
+    for (int j = 0; j < EXP_STEPS / STREAM_NT; ++j) table[j * STREAM_NT + threadIdx.x] = EXP_TABLE.v[j * STREAM_NT + threadIdx.x];
 }
 
 template <class T>
-__global__ void __launch_bounds__(STREAM_NT) sample_weigh_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int slices, int parts_each) {
+__global__ void __launch_bounds__(STREAM_NT) sample_weigh_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int cuts) {
     constexpr int N = Piece<T>::N;
     __shared__ double table[EXP_STEPS];
     __shared__ u64 hist[BINS];
-    const int64_t row = blockIdx.x / slices;
-    const int slice = (int)(blockIdx.x - row * slices), mode = work.state[row].mode;
+    const int64_t row = blockIdx.x / cuts;
+    const int slice = (int)(blockIdx.x - row * cuts), mode = work.state[row].mode;
     if (mode != ROW_SUM && mode != ROW_MASS) return;
+    const float best = work.state[row].best;
     const Source<T> src(scores, a, row);
     const Settings set(a, row);
-    make_table(table, threadIdx.x, STREAM_NT);
-    if (mode == ROW_MASS)
-        for (int b = threadIdx.x; b < BINS; b += STREAM_NT) hist[b] = 0;
-    __syncthreads();
-    const FixedExp weigh(work.state[row].best, set.tau, a.shift, table);
+    const FixedExp weigh(best, set.tau, a.shift, table);
     const u64 least_w = mode == ROW_SUM ? set.least_weight(a.shift) : 0;
-    stream_parts(src, work, row, slice * parts_each, parts_each, [&](const Piece<T>& v, int) {
-        u64 sum = 0;
+    stream_parts(src, work, slice * PARTS_EACH, work.part + row * PARTS, [&](const Piece<T>& v, int) {
+        u64 w[N], sum = 0;
 #pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float z = v.get(e);
-            const u64 w = weigh(z);
-            sum += w >= least_w ? w : 0;
-            if (mode == ROW_MASS && w) atomicAdd(&hist[weigh.bin(z)], w);
+        for (int e = 0; e < N; ++e) w[e] = weigh(v.get(e));
+        if (mode == ROW_MASS) {
+            // no branch between the scores: their chains of dependent steps overlap
+#pragma unroll
+            for (int e = 0; e < N; ++e) atomicAdd(&hist[weigh.bin(v.get(e))], w[e]);
+        } else if (least_w) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = w[e] >= least_w ? w[e] : 0;
         }
+#pragma unroll
+        for (int e = 0; e < N; ++e) sum += w[e];
         return sum;
+    }, [&] {
+        stream_table(table);
+        if (mode == ROW_MASS)
+            for (int b = threadIdx.x; b < BINS; b += STREAM_NT) hist[b] = 0;
+        __syncthreads();
     });
     if (mode != ROW_MASS) return;
     __syncthreads();
     for (int b = threadIdx.x; b < BINS; b += STREAM_NT)
         if (hist[b]) atomicAdd(&work.hist[row * BINS + b], hist[b]);
+}
+
+template <class T>
+__global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int cuts) {
+    constexpr int N = Piece<T>::N;
+    __shared__ double table[EXP_STEPS];
+    __shared__ float member_z[LIST_MAX];
+    __shared__ uint32_t member_at[LIST_MAX];
+    __shared__ uint32_t members, base;
+    const int64_t row = blockIdx.x / cuts;
+    const int slice = (int)(blockIdx.x - row * cuts);
+    RowState& state = work.state[row];
+    if (state.mode != ROW_MASS) return;
+    const float best = state.best;
+    const int b = state.bin;
+    const Source<T> src(scores, a, row);
+    const Settings set(a, row);
+    const FixedExp weigh(best, set.tau, a.shift, table);
+    const u64 least_w = set.least_weight(a.shift);
+    float lo, hi;
+    weigh.bin_range(b, &lo, &hi);
+    stream_parts(src, work, slice * PARTS_EACH, work.part + row * PARTS, [&](const Piece<T>& v, int at) {
+        float top = v.get(0);
+#pragma unroll
+        for (int e = 1; e < N; ++e) top = fmaxf(top, v.get(e));
+        u64 sum = 0;
+        if (!__ballot(top >= lo)) return sum;
+        u64 w[N];
+        bool near = false;
+#pragma unroll
+        for (int e = 0; e < N; ++e) w[e] = weigh(v.get(e));
+#pragma unroll
+        for (int e = 0; e < N; ++e) {
+            const float z = v.get(e);
+            sum += z > hi && w[e] >= least_w ? w[e] : 0;
+            near |= z >= lo && z <= hi;
+        }
+        if (near) {
+            // the bin's own scores, and those beside it that the bin's range takes in
+#pragma unroll
+            for (int e = 0; e < N; ++e) {
+                const float z = v.get(e);
+                if (!(z >= lo && z <= hi)) continue;
+                const int bin = weigh.bin(z);
+                if (bin < b) sum += w[e] >= least_w ? w[e] : 0;
+                else if (bin == b) {
+                    const uint32_t to = atomicAdd(&members, 1u);
+                    if (to < LIST_MAX) { member_z[to] = z; member_at[to] = (uint32_t)(at + e); }
+                }
+            }
+        }
+        return sum;
+    }, [&] {
+        stream_table(table);
+        if (threadIdx.x == 0) members = 0;
+        __syncthreads();
+    });
+    __syncthreads();
+    const uint32_t mine = members;
+    if (threadIdx.x == 0 && mine) base = atomicAdd(&state.members, mine);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < min(mine, (uint32_t)LIST_MAX); i += STREAM_NT) {
+        const uint32_t to = base + i;
+        if (to >= LIST_MAX) break;
+        work.member_z[row * LIST_MAX + to] = member_z[i];
+        work.member_at[row * LIST_MAX + to] = member_at[i];
+    }
+}
+
+template <class T>
+__global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+    __shared__ SampleShared sh;
+    sample_pick(sh, scores, a, work, blockIdx.x);
 }
 
 // The row's parts, of `total` after scan_parts: the one that holds the goal, read again by the first wave.
@@ -1060,12 +1170,12 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_border_ke
     RowState& state = work.state[row];
     const int mode = state.mode, tid = threadIdx.x;
     if (mode != ROW_SUM && mode != ROW_MASS) return;
+    const float best = state.best;
     const Settings set(a, row);
-    if (tid < work.parts) sh.part[tid] = work.part[row * PARTS + tid];
+    const u64 part = tid < work.parts ? work.part[row * PARTS + tid] : 0;
     if (mode == ROW_MASS) {
         for (int b = tid; b < BINS; b += SAMPLE_NT) sh.bin[b] = work.hist[row * BINS + b];
-        const u64 total = block_total(sh, tid < work.parts ? sh.part[tid] : 0);
-        const double target = (double)total * (double)set.top_p;
+        const double target = (double)block_total(sh, part) * (double)set.top_p;
         const u64 least = max((u64)ceil(target), (u64)1);
         find_bin(sh, 0, least, false);
         if (tid == 0) {
@@ -1076,51 +1186,13 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_border_ke
         }
         return;
     }
-    make_table(sh.table, tid, SAMPLE_NT);
+    sh.part[tid] = part;
+    make_table(sh.table);
     const u64 total = scan_parts(sh, work.parts), least_w = set.least_weight(a.shift);
-    const FixedExp weigh(state.best, set.tau, a.shift, sh.table);
+    const FixedExp weigh(best, set.tau, a.shift, sh.table);
     draw_from_parts(sh, Source<T>(scores, a, row), a, work, row, set, total, [&](float z, uint32_t) {
         const u64 w = weigh(z);
         return w >= least_w ? w : (u64)0;
-    });
-}
-
-template <class T>
-__global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int slices, int parts_each) {
-    constexpr int N = Piece<T>::N;
-    __shared__ double table[EXP_STEPS];
-    const int64_t row = blockIdx.x / slices;
-    const int slice = (int)(blockIdx.x - row * slices);
-    RowState& state = work.state[row];
-    if (state.mode != ROW_MASS) return;
-    const Source<T> src(scores, a, row);
-    const Settings set(a, row);
-    make_table(table, threadIdx.x, STREAM_NT);
-    __syncthreads();
-    const FixedExp weigh(state.best, set.tau, a.shift, table);
-    const u64 least_w = set.least_weight(a.shift);
-    const int b = state.bin;
-    float lo, hi;
-    weigh.bin_range(b, &lo, &hi);
-    stream_parts(src, work, row, slice * parts_each, parts_each, [&](const Piece<T>& v, int at) {
-        u64 sum = 0;
-#pragma unroll
-        for (int e = 0; e < N; ++e) {
-            const float z = v.get(e);
-            if (!__ballot(z >= lo)) continue;
-            const int bin = z >= weigh.cut ? weigh.bin(z) : BINS;
-            if (bin < b) {
-                const u64 w = weigh(z);
-                sum += w >= least_w ? w : 0;
-            } else if (bin == b) {
-                const uint32_t to = atomicAdd(&state.members, 1u);
-                if (to < LIST_MAX) {
-                    work.member_z[row * LIST_MAX + to] = z;
-                    work.member_at[row * LIST_MAX + to] = (uint32_t)(at + e);
-                }
-            }
-        }
-        return sum;
     });
 }
 
@@ -1132,42 +1204,43 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_rest_kern
     if (state.mode == ROW_WHOLE || (state.mode == ROW_MASS && state.members > LIST_MAX)) return sample_whole_row(sh, scores, a, row);
     if (state.mode != ROW_MASS) return;
     const Settings set(a, row);
+    const Source<T> src(scores, a, row);
     const int members = (int)state.members;
-    make_table(sh.table, tid, SAMPLE_NT);
+    if (tid < work.parts) sh.part[tid] = work.part[row * PARTS + tid];
     for (int i = tid; i < members; i += SAMPLE_NT) {
         sh.list_z[i] = work.member_z[row * LIST_MAX + i];
         sh.list_at[i] = work.member_at[row * LIST_MAX + i];
     }
-    if (tid < work.parts) sh.part[tid] = work.part[row * PARTS + tid];
-    if (tid == 0) sh.first = 0xffffffffu;
+    make_table(sh.table);
     __syncthreads();
     const FixedExp weigh(state.best, set.tau, a.shift, sh.table);
     const u64 least_w = set.least_weight(a.shift);
+    float cut = -INFINITY;
+    uint32_t tie_end = 0xffffffffu;              // rows at the cut from this one on are out
+    auto weight_at = [&](float z, uint32_t at) {
+        const u64 w = weigh(z);
+        return (z > cut || (z == cut && at < tie_end)) && w >= least_w ? w : (u64)0;
+    };
     float lo, hi;
     weigh.bin_range(state.bin, &lo, &hi);
     u64 above;
-    const float cut = score_of(narrow(sh, [&](auto&& f) {
+    cut = score_of(narrow(sh, [&](auto&& f) {
         for (int i = tid; i < members; i += SAMPLE_NT) {
             const float z = sh.list_z[i];
             f(pattern(z), [&] { return weigh(z); });
         }
     }, pattern(lo), pattern(hi), state.above, state.least, &above));
-    const int64_t ties = ties_within(state.target, above, weigh(cut));
-    const uint32_t tie_end = first_tie_out(sh, [&](auto&& f) {
+    tie_end = first_tie_out(sh, [&](auto&& f) {
         for (int i = tid; i < members; i += SAMPLE_NT)
             if (sh.list_z[i] == cut) f(sh.list_at[i]);
-    }, ties, (uint32_t)a.vocab);
-    auto weight_at = [&](float z, uint32_t at) {
-        const u64 w = weigh(z);
-        return (z > cut || (z == cut && at < tie_end)) && w >= least_w ? w : (u64)0;
-    };
+    }, ties_within(state.target, above, weigh(cut)), (uint32_t)a.vocab);
     __syncthreads();
     for (int i = tid; i < members; i += SAMPLE_NT) {
         const u64 w = weight_at(sh.list_z[i], sh.list_at[i]);
         if (w) atomicAdd(&sh.part[sh.list_at[i] / (uint32_t)work.part_len], w);
     }
     const u64 total = scan_parts(sh, work.parts);
-    draw_from_parts(sh, Source<T>(scores, a, row), a, work, row, set, total, weight_at);
+    draw_from_parts(sh, src, a, work, row, set, total, weight_at);
 }
 
 // Short rows go to one block each: what the other form saves in passes it loses in launches.
@@ -1179,20 +1252,21 @@ template <class T> static int launch_long_rows(const T* z, int64_t n, const Samp
     const int slices = ceil_div(a.vocab, STREAM_NT * Piece<T>::N * STREAM_PIECES);
     hipLaunchKernelGGL(sample_groups_kernel<T>, dim3((unsigned)(n * slices)), dim3(STREAM_NT), 0, s, z, a, w, slices);
     VDB_HIP(hipGetLastError());
+    // whether rows can need their weights, and a border among them
+    const bool all_known = !a.d_temperature && !a.d_top_k && !a.d_top_p && !a.d_min_p;
+    const RowMode mode = mode_of(a.temperature, a.top_k, a.top_p, a.min_p);
+    const bool listed = all_known ? mode == ROW_LIST || mode == ROW_WHOLE
+                                  : (!a.d_temperature && !(a.temperature > 0.0f)) || (!a.d_top_k && a.top_k >= 1) || (!a.d_top_p && a.top_p <= 0.0f);
     hipLaunchKernelGGL(sample_pick_kernel<T>, rows, block, 0, s, z, a, w);
     VDB_HIP(hipGetLastError());
-    const bool settled = (!a.d_temperature && !(a.temperature > 0.0f)) || (!a.d_top_p && a.top_p <= 0.0f) ||
-                         (!a.d_top_k && a.top_k >= 1 && a.top_k <= SAMPLE_NT);      // whatever the scores, but for long ties
-    if (!settled) {
-        // parts a block: few where there are few rows, so that they spread over the chip, else enough to pay for its table
-        const int parts_each = n * w.parts >= (int64_t)2048 * 32 ? 32 : 8, cuts = ceil_div(w.parts, parts_each);
-        const dim3 grid((unsigned)(n * cuts));
-        hipLaunchKernelGGL(sample_weigh_kernel<T>, grid, dim3(STREAM_NT), 0, s, z, a, w, cuts, parts_each);
+    if (!listed) {
+        const int cuts = ceil_div(w.parts, PARTS_EACH);
+        hipLaunchKernelGGL(sample_weigh_kernel<T>, dim3((unsigned)(n * cuts)), dim3(STREAM_NT), 0, s, z, a, w, cuts);
         VDB_HIP(hipGetLastError());
         hipLaunchKernelGGL(sample_border_kernel<T>, rows, block, 0, s, z, a, w);
         VDB_HIP(hipGetLastError());
         if (a.d_top_p || a.top_p < 1.0f) {
-            hipLaunchKernelGGL(sample_above_kernel<T>, grid, dim3(STREAM_NT), 0, s, z, a, w, cuts, parts_each);
+            hipLaunchKernelGGL(sample_above_kernel<T>, dim3((unsigned)(n * cuts)), dim3(STREAM_NT), 0, s, z, a, w, cuts);
             VDB_HIP(hipGetLastError());
         }
     }
