@@ -20,8 +20,11 @@
 
 namespace vdb {
 
-static constexpr int SAMPLE_NT = 1024, SAMPLE_WAVES = SAMPLE_NT / 64;
-static constexpr int LIST_MAX = 2048, LIST_ITEMS = LIST_MAX / SAMPLE_NT, BINS = 2 * SAMPLE_NT, EXP_STEPS = 1024, GROUPS = 64, AHEAD = 4, PAIRS = 256;
+// Passes over a whole row by one block take ROW_NT threads.  Everything else that a block does for a row is a chain of short
+// steps between barriers, and every instruction of such a step costs each wave of a SIMD its turn: FEW_NT threads, two waves
+// a SIMD (one row of 131072 bf16 scores, top-k 400: 23 us; with 256 threads 30, with 1024 27).
+static constexpr int ROW_NT = 1024, ROW_WAVES = ROW_NT / 64, FEW_NT = 512;
+static constexpr int LIST_MAX = 2048, BINS = 2048, EXP_STEPS = 1024, GROUPS = 64, AHEAD = 4, PAIRS = 256;
 typedef unsigned long long u64;
 static constexpr float LOWEST = -3.4028234663852886e38f;
 
@@ -127,7 +130,8 @@ template <class T> struct Source {
 
 // The weight exp((z - best) / tau) as a multiple of 2^-s: with x = (z - best) c, c = 1024 log2(e) / tau, and k = x rounded,
 // 2^(x / 1024) = 2^(k >> 10) table[k & 1023] q(x - k), q a cubic (its remainder is below 2^-50 for |x - k| <= 1/2).  Adding
-// 2^(52 - s) leaves the multiple in the low mantissa bits.  About 18 instructions a score; exp2() of the library takes 40.
+// 2^(52 - s) leaves the multiple in the low mantissa bits.  Nine double instructions, 8 cycles each, and as many others,
+// are what streaming weights is bound by (33.5M of them: 36 us; with 32 entries and degree 5, free of bank conflicts, 41 us).
 struct FixedExp {
     double best, c, round_to;        // round_to = 2^(52 - s)
     float cut;                       // scores below weigh nothing (2^-40 of the best)
@@ -136,22 +140,25 @@ struct FixedExp {
     __device__ __forceinline__ FixedExp(float best_, float tau, int shift, const double* t)
         : best(best_), c(EXP_STEPS * 1.4426950408889634073599 / (double)tau), round_to((double)((u64)1 << (52 - shift))),
           cut((float)fmax((double)best_ - 40.0 * 0.69314718055994530942 * (double)tau, (double)LOWEST)), table(t) {}
-    // scores of bin b lie in [*lo, *hi]; what else does is told apart by its bin
+    // Distances from the best are binned in steps of 1/32 of a power of two.  Scores of bin b lie in [*lo, *hi]; what else
+    // does is told apart by its bin.
     __device__ __forceinline__ void bin_range(int b, float* lo, float* hi) const {
         const double h = best - (32.0 * b - 0.6) / c, l = best - (32.0 * b + 31.6) / c;
         *hi = (float)fmin(best, h + fabs(h) * 2.4e-7);
         *lo = (float)fmax(l - fabs(l) * 2.4e-7, (double)cut);
     }
-    __device__ __forceinline__ int bin(float z) const {              // distance from the best in steps of 1/32 of a power of two
+    __device__ __forceinline__ int bin(float z) const {
         const int k = (int)(uint32_t)__double_as_longlong(fma((double)z - best, c, NEAREST));
-        return (int)min((uint32_t)(-k) >> 5, (uint32_t)(BINS - 1));
+        return (int)min((uint32_t)-k >> 5, (uint32_t)(BINS - 1));
     }
     // the same without the table, for a few scores: exp2() to the last bits of a double
     __device__ __forceinline__ u64 directly(float z) const {
         const double w = exp2(((double)z - best) * (c / EXP_STEPS));
         return z >= cut ? (u64)__double_as_longlong(w + round_to) - (u64)__double_as_longlong(round_to) : 0;
     }
-    __device__ __forceinline__ u64 operator()(float z) const {
+    __device__ __forceinline__ u64 operator()(float z) const { return from(z, cut); }
+    // 0 for scores below `least`, which is not below cut
+    __device__ __forceinline__ u64 from(float z, float least) const {
         constexpr double L = 0.69314718055994530942 / EXP_STEPS;
         const double d = (double)z - best;
         const double a = fma(d, c, NEAREST);
@@ -163,7 +170,7 @@ struct FixedExp {
         const u64 t = (u64)__double_as_longlong(table[k & (EXP_STEPS - 1)]);
         const double scale = __longlong_as_double((long long)(t + ((u64)(uint32_t)(k >> 10) << 52)));
         const u64 r = (u64)__double_as_longlong(fma(scale, q, round_to)) - (u64)__double_as_longlong(round_to);
-        return z >= cut ? r : 0;
+        return z >= least ? r : 0;
     }
 };
 
@@ -172,12 +179,12 @@ struct SampleShared {
     u64 bin[BINS];
     float list_z[LIST_MAX];
     uint32_t list_at[LIST_MAX];
-    u64 part[SAMPLE_WAVES * GROUPS];     // per part of the row, in row order: counts or weights, then their exclusive prefix
+    u64 part[ROW_WAVES * GROUPS];     // per part of the row, in row order: counts or weights, then their exclusive prefix
     u64 pair_sum[PAIRS], pair_w[PAIRS];
     uint32_t pair_rank[PAIRS];
     u64 few_w[64];
     uint32_t few_key[64];
-    u64 red[SAMPLE_WAVES];
+    u64 red[ROW_WAVES];
     u64 found_sum;
     uint32_t found, first, listed, few;
 };
@@ -201,9 +208,9 @@ __device__ __forceinline__ u64 last_lane(u64 v) {
     return ((u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), 63) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, 63);
 }
 __device__ __forceinline__ u64 wave_sum(u64 v) { return last_lane(wave_scan(v)); }
-// (the loops over the waves' sums are unrolled: their loads go out together)
-// exclusive prefix of v over the block; *total = its sum
-__device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* total) {
+// Helpers of a block's first NT threads (the others have ended, or take part elsewhere in no barrier).
+// exclusive prefix of v; *total = its sum
+template <int NT> __device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const u64 inc = wave_scan(v);
     __syncthreads();
@@ -211,37 +218,45 @@ __device__ __forceinline__ u64 block_scan(SampleShared& sh, u64 v, u64* total) {
     __syncthreads();
     u64 all = 0, base = 0;
 #pragma unroll
-    for (int w = 0; w < SAMPLE_WAVES; ++w) {
-        if (w < wave) base += sh.red[w];
-        all += sh.red[w];
+    for (int w = 0; w < NT / 64; ++w) {
+        const u64 r = sh.red[w];
+        base += w < wave ? r : 0;
+        all += r;
     }
     *total = all;
     return base + inc - v;
 }
-__device__ __forceinline__ u64 block_total(SampleShared& sh, u64 v) {
+template <int NT> __device__ __forceinline__ u64 block_total(SampleShared& sh, u64 v) {
     v = wave_sum(v);
     __syncthreads();
     if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = v;
     __syncthreads();
     v = 0;
 #pragma unroll
-    for (int w = 0; w < SAMPLE_WAVES; ++w) v += sh.red[w];
+    for (int w = 0; w < NT / 64; ++w) v += sh.red[w];
     return v;
 }
 // the parts' exclusive prefix in place; -> their sum
-__device__ __forceinline__ u64 scan_parts(SampleShared& sh, int parts) {
+template <int NT> __device__ __forceinline__ u64 scan_parts(SampleShared& sh, int parts) {
+    constexpr int PER = ROW_WAVES * GROUPS / NT;
     __syncthreads();
-    const int tid = threadIdx.x;
-    u64 total;
-    const u64 v = block_scan(sh, tid < parts ? sh.part[tid] : 0, &total);
-    if (tid < parts) sh.part[tid] = v;
+    const int at = threadIdx.x * PER;
+    u64 v[PER], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += v[j] = at + j < parts ? sh.part[at + j] : 0;
+    u64 run = block_scan<NT>(sh, sum, &total);
+#pragma unroll
+    for (int j = 0; j < PER; ++j) {
+        if (at + j < parts) sh.part[at + j] = run;
+        run += v[j];
+    }
     __syncthreads();
     return total;
 }
-__device__ __forceinline__ void clear_bins(SampleShared& sh) {
+template <int NT> __device__ __forceinline__ void clear_bins(SampleShared& sh) {
     __syncthreads();
-    sh.bin[threadIdx.x] = 0;
-    sh.bin[threadIdx.x + SAMPLE_NT] = 0;
+#pragma unroll
+    for (int j = 0; j < BINS / NT; ++j) sh.bin[j * NT + threadIdx.x] = 0;
     __syncthreads();
 }
 // 2^(j / 1024), by exp's series to the last bits of a double
@@ -257,38 +272,47 @@ struct ExpTable {
     }
 };
 __device__ constexpr ExpTable EXP_TABLE{};
-static_assert(EXP_STEPS == SAMPLE_NT, "a thread an entry");
-__device__ __forceinline__ void make_table(double* table) { table[threadIdx.x] = EXP_TABLE.v[threadIdx.x]; }
+template <int NT> __device__ __forceinline__ void make_table(double* table) {
+#pragma unroll
+    for (int j = 0; j < EXP_STEPS / NT; ++j) table[j * NT + threadIdx.x] = EXP_TABLE.v[j * NT + threadIdx.x];
+}
 // the first bin, from the top or from the bottom, at which the running sum, from `above`, reaches target: sh.found its
 // number in that order (BINS: none), sh.found_sum the sum before it
-__device__ static void find_bin(SampleShared& sh, u64 above, u64 target, bool from_top) {
+template <int NT> __device__ __forceinline__ void find_bin(SampleShared& sh, u64 above, u64 target, bool from_top) {
+    constexpr int PER = BINS / NT;
     __syncthreads();
-    const int at = 2 * threadIdx.x;
-    const u64 v0 = sh.bin[from_top ? BINS - 1 - at : at], v1 = sh.bin[from_top ? BINS - 2 - at : at + 1];
-    u64 total;
+    const int at = PER * threadIdx.x;
+    u64 v[PER], sum = 0, total;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) sum += v[j] = sh.bin[from_top ? BINS - 1 - at - j : at + j];
     if (threadIdx.x == 0) sh.found = BINS;
-    u64 run = above + block_scan(sh, v0 + v1, &total);          // its barriers order the write above with those below
-    if (run < target && run + v0 + v1 >= target) {
-        const bool second = run + v0 < target;
-        sh.found = (uint32_t)(at + (second ? 1 : 0));
-        sh.found_sum = run + (second ? v0 : 0);
+    u64 run = above + block_scan<NT>(sh, sum, &total);          // its barriers order the write above with those below
+    if (run < target && run + sum >= target) {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            if (run < target && run + v[j] >= target) {
+                sh.found = (uint32_t)(at + j);
+                sh.found_sum = run;
+            }
+            run += v[j];
+        }
     }
     __syncthreads();
 }
 
 // 11 bits of a search: the part of [*lo, *hi] in which the running sum of the weights, by descending key and from *above,
 // reaches target (false: it does not; nothing changes).  each calls f(key, weight), weight a function.
-template <class Each>
+template <int NT, class Each>
 __device__ __forceinline__ bool narrow_step(SampleShared& sh, Each&& each, uint32_t* lo, uint32_t* hi, u64* above, u64 target) {
     const uint32_t first = *lo, last = *hi;
     const int shift = max(21 - __clz(last - first), 0);
-    clear_bins(sh);
+    clear_bins<NT>(sh);
     each([&](uint32_t key, auto&& weight) {
         if (key < first || key > last) return;
         const u64 v = weight();
         if (v) atomicAdd(&sh.bin[(key - first) >> shift], v);
     });
-    find_bin(sh, *above, target, true);
+    find_bin<NT>(sh, *above, target, true);
     if (sh.found == BINS) return false;
     const uint32_t b = BINS - 1 - sh.found, end = first + ((b + 1) << shift) - 1;
     *above = sh.found_sum;
@@ -299,9 +323,9 @@ __device__ __forceinline__ bool narrow_step(SampleShared& sh, Each&& each, uint3
 // The key among those of each(f) in [lo, hi] at which the running sum of the weights, by descending key and from `above`,
 // reaches target (0 < target; where it is not reached: lo); *sum_above = the sum before it.  What a step leaves is settled at
 // once by a wave that compares all pairs, if it is few.
-template <class Each>
+template <int NT, class Each>
 __device__ __forceinline__ uint32_t narrow(SampleShared& sh, Each&& each, uint32_t lo, uint32_t hi, u64 above, u64 target, u64* sum_above) {
-    while (lo < hi && narrow_step(sh, each, &lo, &hi, &above, target) && lo < hi) {
+    while (lo < hi && narrow_step<NT>(sh, each, &lo, &hi, &above, target) && lo < hi) {
         if (threadIdx.x == 0) sh.few = 0;
         __syncthreads();
         each([&](uint32_t key, auto&& weight) {
@@ -339,11 +363,11 @@ __device__ __forceinline__ uint32_t narrow(SampleShared& sh, Each&& each, uint32
 __device__ __forceinline__ u64 one_each() { return 1; }
 // A bound that no fewer than k of the scores of each(f) reach, and few more: the lower end of the part in which the k-th
 // largest lies.  lowest, best: their range.  -LOWEST where there are fewer than k.
-template <class Each> __device__ __forceinline__ float bound_of(SampleShared& sh, Each&& each, float lowest, float best, int k) {
+template <int NT, class Each> __device__ __forceinline__ float bound_of(SampleShared& sh, Each&& each, float lowest, float best, int k) {
     uint32_t lo = pattern(lowest), hi = pattern(best);
     u64 above = 0;
-    if (!narrow_step(sh, each, &lo, &hi, &above, (u64)k)) return LOWEST;
-    if (hi - lo >= 1u << 16) narrow_step(sh, each, &lo, &hi, &above, (u64)k);        // a range around zero holds most patterns
+    if (!narrow_step<NT>(sh, each, &lo, &hi, &above, (u64)k)) return LOWEST;
+    if (hi - lo >= 1u << 16) narrow_step<NT>(sh, each, &lo, &hi, &above, (u64)k);        // a range around zero holds most patterns
     return score_of(lo);
 }
 // lanes with `want` add to the list; the number of all that wanted is in sh.listed
@@ -359,20 +383,25 @@ __device__ __forceinline__ void append(SampleShared& sh, bool want, float z, uin
         sh.list_at[from] = at;
     }
 }
-// smallest and largest over the block (-inf: nothing there), of values that are not NaN
-__device__ __forceinline__ void block_range(SampleShared& sh, float& lowest, float& best) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        best = fmaxf(best, __shfl_xor(best, o));
-        lowest = fminf(lowest, __shfl_xor(lowest, o));
-    }
+// smallest and largest over the block, of values that are not NaN
+template <int CTRL, int ROWS> __device__ __forceinline__ float moved(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(v), __float_as_int(v), CTRL, ROWS, 0xf, false));
+}
+template <int NT> __device__ __forceinline__ void block_range(SampleShared& sh, float& lowest, float& best) {
+#define VDB_RANGE_STEP(CTRL, ROWS) { best = fmaxf(best, moved<CTRL, ROWS>(best)); lowest = fminf(lowest, moved<CTRL, ROWS>(lowest)); }
+    VDB_RANGE_STEP(0x111, 0xf) VDB_RANGE_STEP(0x112, 0xf) VDB_RANGE_STEP(0x114, 0xf) VDB_RANGE_STEP(0x118, 0xf)      // as wave_scan
+    VDB_RANGE_STEP(0x142, 0xa) VDB_RANGE_STEP(0x143, 0xc)
+#undef VDB_RANGE_STEP
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.red[threadIdx.x >> 6] = ((u64)__float_as_uint(lowest) << 32) | __float_as_uint(best);
+    if ((threadIdx.x & 63) == 63) sh.red[threadIdx.x >> 6] = ((u64)__float_as_uint(lowest) << 32) | __float_as_uint(best);
     __syncthreads();
+    best = -INFINITY;
+    lowest = INFINITY;
 #pragma unroll
-    for (int w = 0; w < SAMPLE_WAVES; ++w) {
-        best = fmaxf(best, __uint_as_float((uint32_t)sh.red[w]));
-        lowest = fminf(lowest, __uint_as_float((uint32_t)(sh.red[w] >> 32)));
+    for (int w = 0; w < NT / 64; ++w) {
+        const u64 r = sh.red[w];
+        best = fmaxf(best, __uint_as_float((uint32_t)r));
+        lowest = fminf(lowest, __uint_as_float((uint32_t)(r >> 32)));
     }
 }
 
@@ -390,17 +419,18 @@ __device__ __forceinline__ int64_t ties_within(double target, u64 above, u64 w) 
 }
 
 // Of the rows at a cut, each(f) calling f(row), the first `ties` remain: the first one that is out (or 2^32 - 1).
-template <class Each> __device__ __forceinline__ uint32_t first_tie_out(SampleShared& sh, Each&& each, int64_t ties, uint32_t vocab) {
+template <int NT, class Each> __device__ __forceinline__ uint32_t first_tie_out(SampleShared& sh, Each&& each, int64_t ties, uint32_t vocab) {
     if (ties == INT64_MAX) return 0xffffffffu;
     u64 count = 0, ignored;
     each([&](uint32_t) { ++count; });
-    if ((int64_t)block_total(sh, count) <= ties) return 0xffffffffu;
-    return ~narrow(sh, [&](auto&& f) { each([&](uint32_t at) { f(~at, one_each); }); }, ~vocab, 0xffffffffu, 0, (u64)ties + 1, &ignored);
+    if ((int64_t)block_total<NT>(sh, count) <= ties) return 0xffffffffu;
+    return ~narrow<NT>(sh, [&](auto&& f) { each([&](uint32_t at) { f(~at, one_each); }); }, ~vocab, 0xffffffffu, 0, (u64)ties + 1, &ignored);
 }
 
 // ---------------------------------------------------------------- the draw from a list
 // `listed` <= LIST_MAX scores and their rows in sh.list_*, in any order, among them all that remain.
-__device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& a, int64_t row, const Settings& set, const FixedExp& weigh, int listed) {
+template <int NT> __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& a, int64_t row, const Settings& set, const FixedExp& weigh, int listed) {
+    constexpr int LIST_ITEMS = LIST_MAX / NT;
     const int tid = threadIdx.x;
     const u64 least_w = set.least_weight(a.shift);
     if (listed <= PAIRS) {
@@ -408,7 +438,7 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
         // comparing all pairs, the block's threads in slices of the list
         int log_width = 6;
         while ((1 << log_width) < listed) ++log_width;
-        const int i = tid & ((1 << log_width) - 1), slice = tid >> log_width, slices = SAMPLE_NT >> log_width;
+        const int i = tid & ((1 << log_width) - 1), slice = tid >> log_width, slices = NT >> log_width;
         const float zi = i < listed ? sh.list_z[i] : 0.0f;
         const uint32_t at = i < listed ? sh.list_at[i] : 0;
         u64 w = 0;
@@ -433,13 +463,13 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
         __syncthreads();
         if (set.by_count() && tid < listed && sh.pair_rank[tid] >= (uint32_t)set.top_k) w = 0;
         if (set.by_mass()) {
-            const double target = (double)block_total(sh, w) * (double)set.top_p;
+            const double target = (double)block_total<NT>(sh, w) * (double)set.top_p;
             if (tid < listed && sh.pair_rank[tid] > 0 && !((double)sh.pair_sum[tid] < target)) w = 0;
         }
         if (w < least_w) w = 0;
         __syncthreads();
         if (tid < PAIRS) { sh.pair_w[tid] = w; sh.pair_sum[tid] = 0; }
-        const u64 all = block_total(sh, w), least = set.goal(all);
+        const u64 all = block_total<NT>(sh, w), least = set.goal(all);
         if (i < listed) {
             u64 before = 0;
             for (int j = slice; j < listed; j += slices)
@@ -450,14 +480,14 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
         if (tid < listed && w && sh.pair_sum[tid] < least && sh.pair_sum[tid] + w >= least) write_draw(a, row, at, w, all);
         return;
     }
-    make_table(sh.table);
+    make_table<NT>(sh.table);
     __syncthreads();
     u64 w[LIST_ITEMS];
     float z[LIST_ITEMS];
     uint32_t at[LIST_ITEMS];
 #pragma unroll
     for (int q = 0; q < LIST_ITEMS; ++q) {
-        const int i = q * SAMPLE_NT + tid;
+        const int i = q * NT + tid;
         z[q] = i < listed ? sh.list_z[i] : -INFINITY;
         at[q] = i < listed ? sh.list_at[i] : 0;
         w[q] = weigh(z[q]);
@@ -470,11 +500,11 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
         best = fmaxf(best, z[q]);
         if (z[q] > -INFINITY) lowest = fminf(lowest, z[q]);
     }
-    block_range(sh, lowest, best);
+    block_range<NT>(sh, lowest, best);
     const uint32_t bottom = pattern(lowest), top = pattern(best);
     if (set.by_count() && set.top_k < listed) {
         u64 above;
-        cut = score_of(narrow(sh, [&](auto&& f) {
+        cut = score_of(narrow<NT>(sh, [&](auto&& f) {
 #pragma unroll
             for (int q = 0; q < LIST_ITEMS; ++q) f(pattern(z[q]), one_each);
         }, bottom, top, 0, (u64)set.top_k, &above));
@@ -484,13 +514,13 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
         u64 sum = 0;
 #pragma unroll
         for (int q = 0; q < LIST_ITEMS; ++q) sum += z[q] > cut ? w[q] : 0;
-        const u64 over = block_total(sh, sum), w_cut = ties < INT64_MAX ? weigh(cut) : 0;
+        const u64 over = block_total<NT>(sh, sum), w_cut = ties < INT64_MAX ? weigh(cut) : 0;
         const double target = (double)(over + w_cut * (u64)(ties < INT64_MAX ? ties : 0)) * (double)set.top_p;
         const u64 least = max((u64)ceil(target), (u64)1);
         if (over >= least) {
             u64 above;
             const float floor_z = cut;
-            cut = score_of(narrow(sh, [&](auto&& f) {
+            cut = score_of(narrow<NT>(sh, [&](auto&& f) {
 #pragma unroll
                 for (int q = 0; q < LIST_ITEMS; ++q)
                     if (z[q] > floor_z) f(pattern(z[q]), [&] { return w[q]; });
@@ -500,7 +530,7 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
             ties = min(ties, ties_within(target, over, w_cut));
         }
     }
-    const uint32_t tie_end = first_tie_out(sh, [&](auto&& f) {
+    const uint32_t tie_end = first_tie_out<NT>(sh, [&](auto&& f) {
 #pragma unroll
         for (int q = 0; q < LIST_ITEMS; ++q)
             if (z[q] == cut) f(at[q]);
@@ -511,10 +541,10 @@ __device__ __forceinline__ void draw_listed(SampleShared& sh, const SampleArgs& 
         if (!(z[q] > cut || (z[q] == cut && at[q] < tie_end)) || w[q] < least_w) w[q] = 0;
         sum += w[q];
     }
-    const u64 all = block_total(sh, sum);
+    const u64 all = block_total<NT>(sh, sum);
     u64 before;
     // the row, from the first, at which the running sum reaches the goal
-    const uint32_t drawn = ~narrow(sh, [&](auto&& f) {
+    const uint32_t drawn = ~narrow<NT>(sh, [&](auto&& f) {
 #pragma unroll
         for (int q = 0; q < LIST_ITEMS; ++q)
             if (w[q]) f(~at[q], [&] { return w[q]; });
@@ -567,15 +597,15 @@ template <class T> struct RowPasses {
     int steps, per_group, groups, parts, share;
     __device__ __forceinline__ RowPasses(const Source<T>& s)
         : src(s), tid(threadIdx.x), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) {
-        steps = ((src.vocab + SAMPLE_WAVES - 1) / SAMPLE_WAVES + 64 * N - 1) / (64 * N);
+        steps = ((src.vocab + ROW_WAVES - 1) / ROW_WAVES + 64 * N - 1) / (64 * N);
         per_group = (steps + GROUPS - 1) / GROUPS;
         groups = (steps + per_group - 1) / per_group;
-        parts = SAMPLE_WAVES * groups;
+        parts = ROW_WAVES * groups;
         share = steps * 64 * N;
     }
     // every score, in no order: f(z)
     template <class F> __device__ __forceinline__ void each(F&& f) const {
-        stream_pieces(src, 0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; },
+        stream_pieces(src, 0, (src.vocab + ROW_NT * N - 1) / (ROW_NT * N), [&](int t) { return (t * ROW_NT + tid) * N; },
                       [&](int, int, const Piece<T>& v) {
 #pragma unroll
                           for (int e = 0; e < N; ++e) f(v.get(e));
@@ -597,7 +627,7 @@ template <class T> struct RowPasses {
                 sum = 0;
             }
         });
-        return scan_parts(sh, parts);
+        return scan_parts<ROW_NT>(sh, parts);
     }
     // the parts of the wave that hold(sum before, sum up to): f(sum before, group)
     template <class Hold, class F> __device__ __forceinline__ void parts_that(const SampleShared& sh, u64 total, Hold&& hold, F&& f) const {
@@ -612,7 +642,7 @@ template <class T> struct RowPasses {
         __syncthreads();
         if (tid == 0) sh.listed = 0;
         __syncthreads();
-        stream_pieces(src, 0, (src.vocab + SAMPLE_NT * N - 1) / (SAMPLE_NT * N), [&](int t) { return (t * SAMPLE_NT + tid) * N; },
+        stream_pieces(src, 0, (src.vocab + ROW_NT * N - 1) / (ROW_NT * N), [&](int t) { return (t * ROW_NT + tid) * N; },
                       [&](int, int at, const Piece<T>& v) {
                           float top = v.get(0);
 #pragma unroll
@@ -636,7 +666,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
     pass.each([&](float z) { mine = fmaxf(mine, z); });
     float best = mine, lowest = mine > -INFINITY ? mine : INFINITY;
     if (tid == 0) sh.first = 0xffffffffu;
-    block_range(sh, lowest, best);
+    block_range<ROW_NT>(sh, lowest, best);
     if (best == -INFINITY) {
         if (tid == 0) write_certain(a, row, -1);
         return;
@@ -645,7 +675,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
         uint32_t at = 0xffffffffu;
         if (mine == best) {
 #pragma unroll 1
-            for (int i = tid * N; i < pass.src.vocab && at == 0xffffffffu; i += SAMPLE_NT * N) {
+            for (int i = tid * N; i < pass.src.vocab && at == 0xffffffffu; i += ROW_NT * N) {
                 Piece<T> v = pass.src.load(i);
                 pass.src.finish(v, pass.src.bits(i));
 #pragma unroll
@@ -668,16 +698,19 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
 
     // ---- few rows can remain: a list of them
     float thr = -INFINITY;
-    if (set.by_count() && set.top_k <= SAMPLE_NT) {
-        thr = bound_of(sh, [&](auto&& f) { f(pattern(mine), one_each); }, lowest, best, set.top_k);
+    if (set.by_count() && set.top_k <= ROW_NT) {
+        thr = bound_of<ROW_NT>(sh, [&](auto&& f) { f(pattern(mine), one_each); }, lowest, best, set.top_k);
     } else if (!set.by_count() && !set.by_mass() && least_w) {
         thr = set.min_p_bound(best);
     }
     if (thr > -INFINITY) {
         const int listed = pass.compact(sh, thr);
-        if (listed <= LIST_MAX) return draw_listed(sh, a, row, set, weigh, listed);
+        if (listed <= LIST_MAX) {
+            if (tid >= FEW_NT) return;                           // barriers wait for the waves that have not ended
+            return draw_listed<FEW_NT>(sh, a, row, set, weigh, listed);
+        }
     }
-    make_table(sh.table);                        // the next barrier is clear_bins' or sum_parts'
+    make_table<ROW_NT>(sh.table);                        // the next barrier is clear_bins' or sum_parts'
 
     // ---- the lowest score that remains (cut), and how many of the rows at it
     float cut = -INFINITY;
@@ -685,7 +718,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
     // The score, from the best, at which the running sum of value(z) reaches target(total); false where scores that weigh
     // anything do not reach it.
     auto find_cut = [&](auto&& value, auto&& target, float* at, u64* above) {
-        clear_bins(sh);
+        clear_bins<ROW_NT>(sh);
         u64 sum = 0;
         pass.each([&](float z) {
             if (z >= weigh.cut) {
@@ -694,8 +727,8 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
                 if (v) atomicAdd(&sh.bin[weigh.bin(z)], v);
             }
         });
-        const u64 least = target(block_total(sh, sum));
-        find_bin(sh, 0, least, false);
+        const u64 least = target(block_total<ROW_NT>(sh, sum));
+        find_bin<ROW_NT>(sh, 0, least, false);
         const int b = (int)sh.found;
         if (b == BINS) return false;
         const u64 before = sh.found_sum;
@@ -713,9 +746,9 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
         __syncthreads();
         const int members = (int)sh.found;
         __syncthreads();
-        *at = score_of(narrow(sh, [&](auto&& f) {
+        *at = score_of(narrow<ROW_NT>(sh, [&](auto&& f) {
             if (members <= LIST_MAX) {
-                for (int i = tid; i < members; i += SAMPLE_NT) {
+                for (int i = tid; i < members; i += ROW_NT) {
                     const float z = sh.list_z[i];
                     f(pattern(z), [&] { return value(z); });
                 }
@@ -813,7 +846,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
     });
 }
 
-template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_kernel(const T* __restrict__ scores, SampleArgs a) {
+template <class T> __global__ void __launch_bounds__(ROW_NT) sample_kernel(const T* __restrict__ scores, SampleArgs a) {
     __shared__ SampleShared sh;
     sample_whole_row(sh, scores, a, blockIdx.x);
 }
@@ -836,7 +869,7 @@ struct RowState {
     int mode, bin;
     uint32_t members;
 };
-static constexpr int PARTS = SAMPLE_WAVES * GROUPS;                 // at most, per row
+static constexpr int PARTS = ROW_WAVES * GROUPS;                 // at most, per row
 static constexpr int PARTS_EACH = 4 * (STREAM_NT / 64);             // parts of a streaming block: four a wave
 struct SampleWork {
     float* group_max; int groups;    // [n][groups]
@@ -869,7 +902,7 @@ static SampleWork sample_work(void* base, int64_t n, int64_t vocab) {
 // What a row's settings make of it, before its scores are seen.  Min-p alone mostly leaves few rows where it is 1/64 or more.
 __host__ __device__ static inline RowMode mode_of(float tau, int top_k, float top_p, float min_p) {
     if (!(tau > 0.0f) || top_k == 1 || top_p <= 0.0f) return ROW_LIST;
-    if (top_k > 1) return top_k <= SAMPLE_NT ? ROW_LIST : ROW_WHOLE;
+    if (top_k > 1) return top_k <= LIST_MAX / 2 ? ROW_LIST : ROW_WHOLE;
     if (top_p < 1.0f) return ROW_MASS;
     return min_p >= 0.015625f ? ROW_LIST : ROW_SUM;
 }
@@ -904,23 +937,22 @@ __global__ void __launch_bounds__(STREAM_NT) sample_groups_kernel(const T* __res
     }
 }
 
-// the smallest and the largest of a row's group maxima; a contiguous run [g0, g1) of groups a thread
-struct GroupRun {
+// A row's group maxima, every FEW_NT-th of them a thread's: the first HELD in registers (rows of up to 131072 scores), the
+// others read again in each pass.
+struct GroupMaxima {
+    static constexpr int HELD = 4096 / FEW_NT;
     const float* max;
-    int g0, g1;
-    __device__ __forceinline__ GroupRun(const SampleWork& work, int64_t row) : max(work.group_max + row * work.groups) {
-        const int per = (work.groups + SAMPLE_NT - 1) / SAMPLE_NT;
-        g0 = min((int)threadIdx.x * per, work.groups);
-        g1 = min(g0 + per, work.groups);
+    int groups;
+    float held[HELD];
+    __device__ __forceinline__ GroupMaxima(const SampleWork& work, int64_t row) : max(work.group_max + row * work.groups), groups(work.groups) {
+#pragma unroll
+        for (int q = 0; q < HELD; ++q) held[q] = q * FEW_NT + (int)threadIdx.x < groups ? max[q * FEW_NT + threadIdx.x] : -INFINITY;
     }
-    __device__ __forceinline__ void range(float& lowest, float& best) const {
-        best = -INFINITY;
-        lowest = INFINITY;
-        for (int g = g0; g < g1; ++g) {
-            const float m = max[g];
-            best = fmaxf(best, m);
-            if (m > -INFINITY) lowest = fminf(lowest, m);
-        }
+    // f(group, maximum)
+    template <class F> __device__ __forceinline__ void each(F&& f) const {
+#pragma unroll
+        for (int q = 0; q < HELD; ++q) f(q * FEW_NT + (int)threadIdx.x, held[q]);
+        for (int g = HELD * FEW_NT + threadIdx.x; g < groups; g += FEW_NT) f(g, max[g]);
     }
 };
 
@@ -928,23 +960,24 @@ template <class T> __device__ __forceinline__ void sample_pick(SampleShared& sh,
     const Source<T> src(scores, a, row);
     const Settings set(a, row);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const GroupRun groups(work, row);
-    const float* group_max = groups.max;
-    const int g0 = groups.g0, g1 = groups.g1;
-    float best, lowest;
-    groups.range(lowest, best);
+    const GroupMaxima groups(work, row);
+    float best = -INFINITY, lowest = INFINITY;
+    groups.each([&](int, float m) {
+        best = fmaxf(best, m);
+        if (m > -INFINITY) lowest = fminf(lowest, m);
+    });
     const float mine = best;
     if (tid == 0) { sh.first = 0xffffffffu; sh.listed = sh.found = 0; }
-    block_range(sh, lowest, best);
+    block_range<FEW_NT>(sh, lowest, best);
     if (best == -INFINITY) {
         if (tid == 0) write_certain(a, row, -1);
         return;
     }
     if (set.first_of_best()) {
         if (mine == best) {
-            int g = g0;
-            while (group_max[g] != best) ++g;
-            atomicMin(&sh.first, (uint32_t)g);
+            uint32_t first = 0xffffffffu;
+            groups.each([&](int g, float m) { if (m == best) first = min(first, (uint32_t)g); });
+            atomicMin(&sh.first, first);
         }
         __syncthreads();
         if (tid < GROUP) {
@@ -957,35 +990,40 @@ template <class T> __device__ __forceinline__ void sample_pick(SampleShared& sh,
     const int mode = best == INFINITY ? ROW_WHOLE : mode_of(set.tau, set.top_k, set.top_p, set.min_p);
     if (mode == ROW_LIST) {
         const FixedExp weigh(best, set.tau, a.shift, sh.table);
-        const float thr = !set.by_count() ? set.min_p_bound(best) : bound_of(sh, [&](auto&& f) {
-            for (int g = g0; g < g1; ++g) f(pattern(group_max[g]), one_each);
+        const float thr = !set.by_count() ? set.min_p_bound(best) : bound_of<FEW_NT>(sh, [&](auto&& f) {
+            groups.each([&](int, float m) { f(pattern(m), one_each); });
         }, lowest, best, set.top_k);
         // the groups that reach the bound, and their scores that do
         uint32_t* group = (uint32_t*)sh.bin;
         __syncthreads();
         if (tid == 0) sh.found = 0;
         __syncthreads();
-        for (int g = g0; g < g1; ++g)
-            if (group_max[g] >= thr) {
-                const uint32_t i = atomicAdd(&sh.found, 1u);
-                if (i < LIST_MAX) group[i] = (uint32_t)g;
-            }
+        groups.each([&](int g, float m) {
+            if (!(m >= thr)) return;
+            const uint32_t i = atomicAdd(&sh.found, 1u);
+            if (i < LIST_MAX) group[i] = (uint32_t)g;
+        });
         __syncthreads();
         const int found = (int)sh.found;
         if (found <= LIST_MAX) {
-            // 64 scores a wave, two groups, two such at a time
-            for (int c = 2 * wave; 2 * c < found; c += 2 * SAMPLE_WAVES) {
-                const int k0 = 2 * c + (lane >> 5), k1 = k0 + 2;
-                const int at0 = k0 < found ? (int)group[k0] * GROUP + (lane & (GROUP - 1)) : src.vocab;
-                const int at1 = k1 < found ? (int)group[k1] * GROUP + (lane & (GROUP - 1)) : src.vocab;
-                const float z0 = src.one(at0), z1 = src.one(at1);
-                append(sh, z0 >= thr, z0, (uint32_t)at0);
-                append(sh, z1 >= thr, z1, (uint32_t)at1);
+            // a piece a lane, two at a time: GROUP / N lanes a group
+            constexpr int N = Piece<T>::N, LANES = GROUP / N, WAVE = 64 / LANES;
+            for (int k0 = wave * WAVE + lane / LANES; k0 - lane / LANES < found; k0 += 2 * WAVE * (FEW_NT / 64)) {
+                const int k1 = k0 + WAVE * (FEW_NT / 64);
+                const int at0 = k0 < found ? (int)group[k0] * GROUP + (lane % LANES) * N : src.vocab;
+                const int at1 = k1 < found ? (int)group[k1] * GROUP + (lane % LANES) * N : src.vocab;
+                Piece<T> x0 = src.load(at0), x1 = src.load(at1);
+                src.finish(x0, src.bits(at0));
+                src.finish(x1, src.bits(at1));
+#pragma unroll
+                for (int e = 0; e < N; ++e) append(sh, x0.get(e) >= thr, x0.get(e), (uint32_t)(at0 + e));
+#pragma unroll
+                for (int e = 0; e < N; ++e) append(sh, x1.get(e) >= thr, x1.get(e), (uint32_t)(at1 + e));
             }
             __syncthreads();
             const int listed = (int)sh.listed;
             __syncthreads();
-            if (listed <= LIST_MAX) return draw_listed(sh, a, row, set, weigh, listed);
+            if (listed <= LIST_MAX) return draw_listed<FEW_NT>(sh, a, row, set, weigh, listed);
         }
     }
     if (tid == 0) {
@@ -1010,11 +1048,6 @@ __device__ __forceinline__ void stream_parts(const Source<T>& src, const SampleW
                       sum = 0;
                   }, prologue);
 }
-__device__ __forceinline__ void stream_table(double* table) {
-#pragma unroll
-    for (int j = 0; j < EXP_STEPS / STREAM_NT; ++j) table[j * STREAM_NT + threadIdx.x] = EXP_TABLE.v[j * STREAM_NT + threadIdx.x];
-}
-
 template <class T>
 __global__ void __launch_bounds__(STREAM_NT) sample_weigh_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int cuts) {
     constexpr int N = Piece<T>::N;
@@ -1044,7 +1077,7 @@ __global__ void __launch_bounds__(STREAM_NT) sample_weigh_kernel(const T* __rest
         for (int e = 0; e < N; ++e) sum += w[e];
         return sum;
     }, [&] {
-        stream_table(table);
+        make_table<STREAM_NT>(table);
         if (mode == ROW_MASS)
             for (int b = threadIdx.x; b < BINS; b += STREAM_NT) hist[b] = 0;
         __syncthreads();
@@ -1074,6 +1107,7 @@ __global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __rest
     const u64 least_w = set.least_weight(a.shift);
     float lo, hi;
     weigh.bin_range(b, &lo, &hi);
+    const float beyond = score_of(pattern(hi) + 1);              // the next larger score
     stream_parts(src, work, slice * PARTS_EACH, work.part + row * PARTS, [&](const Piece<T>& v, int at) {
         float top = v.get(0);
 #pragma unroll
@@ -1083,12 +1117,15 @@ __global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __rest
         u64 w[N];
         bool near = false;
 #pragma unroll
-        for (int e = 0; e < N; ++e) w[e] = weigh(v.get(e));
+        for (int e = 0; e < N; ++e) w[e] = weigh.from(v.get(e), beyond);
+        if (least_w) {
+#pragma unroll
+            for (int e = 0; e < N; ++e) w[e] = w[e] >= least_w ? w[e] : 0;
+        }
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            const float z = v.get(e);
-            sum += z > hi && w[e] >= least_w ? w[e] : 0;
-            near |= z >= lo && z <= hi;
+            sum += w[e];
+            near |= v.get(e) >= lo && v.get(e) <= hi;
         }
         if (near) {
             // the bin's own scores, and those beside it that the bin's range takes in
@@ -1097,8 +1134,10 @@ __global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __rest
                 const float z = v.get(e);
                 if (!(z >= lo && z <= hi)) continue;
                 const int bin = weigh.bin(z);
-                if (bin < b) sum += w[e] >= least_w ? w[e] : 0;
-                else if (bin == b) {
+                if (bin < b) {
+                    const u64 w_e = weigh(z);
+                    sum += w_e >= least_w ? w_e : 0;
+                } else if (bin == b) {
                     const uint32_t to = atomicAdd(&members, 1u);
                     if (to < LIST_MAX) { member_z[to] = z; member_at[to] = (uint32_t)(at + e); }
                 }
@@ -1106,7 +1145,7 @@ __global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __rest
         }
         return sum;
     }, [&] {
-        stream_table(table);
+        make_table<STREAM_NT>(table);
         if (threadIdx.x == 0) members = 0;
         __syncthreads();
     });
@@ -1123,7 +1162,7 @@ __global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __rest
 }
 
 template <class T>
-__global__ void __launch_bounds__(SAMPLE_NT) sample_pick_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+__global__ void __launch_bounds__(FEW_NT) sample_pick_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
     __shared__ SampleShared sh;
     sample_pick(sh, scores, a, work, blockIdx.x);
 }
@@ -1135,10 +1174,10 @@ __device__ __forceinline__ void draw_from_parts(SampleShared& sh, const Source<T
     constexpr int N = Piece<T>::N;
     const int tid = threadIdx.x, lane = tid & 63;
     const u64 least = set.goal(total);
-    if (tid < work.parts) {
-        const u64 from = sh.part[tid], to = tid + 1 < work.parts ? sh.part[tid + 1] : total;
+    for (int i = tid; i < work.parts; i += FEW_NT) {
+        const u64 from = sh.part[i], to = i + 1 < work.parts ? sh.part[i + 1] : total;
         if (from < least && to >= least) {
-            sh.found = (uint32_t)tid;
+            sh.found = (uint32_t)i;
             sh.found_sum = from;
         }
     }
@@ -1164,7 +1203,7 @@ __device__ __forceinline__ void draw_from_parts(SampleShared& sh, const Source<T
     }
 }
 
-template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_border_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+template <class T> __global__ void __launch_bounds__(FEW_NT) sample_border_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
     __shared__ SampleShared sh;
     const int64_t row = blockIdx.x;
     RowState& state = work.state[row];
@@ -1172,12 +1211,13 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_border_ke
     if (mode != ROW_SUM && mode != ROW_MASS) return;
     const float best = state.best;
     const Settings set(a, row);
-    const u64 part = tid < work.parts ? work.part[row * PARTS + tid] : 0;
+    u64 part = 0;
+    for (int i = tid; i < work.parts; i += FEW_NT) part += sh.part[i] = work.part[row * PARTS + i];
     if (mode == ROW_MASS) {
-        for (int b = tid; b < BINS; b += SAMPLE_NT) sh.bin[b] = work.hist[row * BINS + b];
-        const double target = (double)block_total(sh, part) * (double)set.top_p;
+        for (int b = tid; b < BINS; b += FEW_NT) sh.bin[b] = work.hist[row * BINS + b];
+        const double target = (double)block_total<FEW_NT>(sh, part) * (double)set.top_p;
         const u64 least = max((u64)ceil(target), (u64)1);
-        find_bin(sh, 0, least, false);
+        find_bin<FEW_NT>(sh, 0, least, false);
         if (tid == 0) {
             state.above = sh.found_sum;
             state.least = least;
@@ -1186,9 +1226,8 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_border_ke
         }
         return;
     }
-    sh.part[tid] = part;
-    make_table(sh.table);
-    const u64 total = scan_parts(sh, work.parts), least_w = set.least_weight(a.shift);
+    make_table<FEW_NT>(sh.table);
+    const u64 total = scan_parts<FEW_NT>(sh, work.parts), least_w = set.least_weight(a.shift);
     const FixedExp weigh(best, set.tau, a.shift, sh.table);
     draw_from_parts(sh, Source<T>(scores, a, row), a, work, row, set, total, [&](float z, uint32_t) {
         const u64 w = weigh(z);
@@ -1196,22 +1235,22 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_border_ke
     });
 }
 
-template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_rest_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+template <class T> __global__ void __launch_bounds__(ROW_NT) sample_rest_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
     __shared__ SampleShared sh;
     const int64_t row = blockIdx.x;
     const RowState state = work.state[row];
     const int tid = threadIdx.x;
     if (state.mode == ROW_WHOLE || (state.mode == ROW_MASS && state.members > LIST_MAX)) return sample_whole_row(sh, scores, a, row);
-    if (state.mode != ROW_MASS) return;
+    if (state.mode != ROW_MASS || tid >= FEW_NT) return;         // barriers wait for the waves that have not ended
     const Settings set(a, row);
     const Source<T> src(scores, a, row);
     const int members = (int)state.members;
-    if (tid < work.parts) sh.part[tid] = work.part[row * PARTS + tid];
-    for (int i = tid; i < members; i += SAMPLE_NT) {
+    for (int i = tid; i < work.parts; i += FEW_NT) sh.part[i] = work.part[row * PARTS + i];
+    for (int i = tid; i < members; i += FEW_NT) {
         sh.list_z[i] = work.member_z[row * LIST_MAX + i];
         sh.list_at[i] = work.member_at[row * LIST_MAX + i];
     }
-    make_table(sh.table);
+    make_table<FEW_NT>(sh.table);
     __syncthreads();
     const FixedExp weigh(state.best, set.tau, a.shift, sh.table);
     const u64 least_w = set.least_weight(a.shift);
@@ -1224,22 +1263,22 @@ template <class T> __global__ void __launch_bounds__(SAMPLE_NT) sample_rest_kern
     float lo, hi;
     weigh.bin_range(state.bin, &lo, &hi);
     u64 above;
-    cut = score_of(narrow(sh, [&](auto&& f) {
-        for (int i = tid; i < members; i += SAMPLE_NT) {
+    cut = score_of(narrow<FEW_NT>(sh, [&](auto&& f) {
+        for (int i = tid; i < members; i += FEW_NT) {
             const float z = sh.list_z[i];
             f(pattern(z), [&] { return weigh(z); });
         }
     }, pattern(lo), pattern(hi), state.above, state.least, &above));
-    tie_end = first_tie_out(sh, [&](auto&& f) {
-        for (int i = tid; i < members; i += SAMPLE_NT)
+    tie_end = first_tie_out<FEW_NT>(sh, [&](auto&& f) {
+        for (int i = tid; i < members; i += FEW_NT)
             if (sh.list_z[i] == cut) f(sh.list_at[i]);
     }, ties_within(state.target, above, weigh(cut)), (uint32_t)a.vocab);
     __syncthreads();
-    for (int i = tid; i < members; i += SAMPLE_NT) {
+    for (int i = tid; i < members; i += FEW_NT) {
         const u64 w = weight_at(sh.list_z[i], sh.list_at[i]);
         if (w) atomicAdd(&sh.part[sh.list_at[i] / (uint32_t)work.part_len], w);
     }
-    const u64 total = scan_parts(sh, work.parts);
+    const u64 total = scan_parts<FEW_NT>(sh, work.parts);
     draw_from_parts(sh, src, a, work, row, set, total, weight_at);
 }
 
@@ -1248,7 +1287,7 @@ static bool by_whole_chip(int64_t vocab) { return vocab >= 16384; }
 static const int64_t SAMPLE_BATCH = 1024;           // rows at a time by the whole chip: bounds the workspace (56 MB at 131072 scores)
 
 template <class T> static int launch_long_rows(const T* z, int64_t n, const SampleArgs& a, const SampleWork& w, hipStream_t s) {
-    const dim3 rows((unsigned)n), block(SAMPLE_NT);
+    const dim3 rows((unsigned)n), few(FEW_NT);
     const int slices = ceil_div(a.vocab, STREAM_NT * Piece<T>::N * STREAM_PIECES);
     hipLaunchKernelGGL(sample_groups_kernel<T>, dim3((unsigned)(n * slices)), dim3(STREAM_NT), 0, s, z, a, w, slices);
     VDB_HIP(hipGetLastError());
@@ -1257,27 +1296,27 @@ template <class T> static int launch_long_rows(const T* z, int64_t n, const Samp
     const RowMode mode = mode_of(a.temperature, a.top_k, a.top_p, a.min_p);
     const bool listed = all_known ? mode == ROW_LIST || mode == ROW_WHOLE
                                   : (!a.d_temperature && !(a.temperature > 0.0f)) || (!a.d_top_k && a.top_k >= 1) || (!a.d_top_p && a.top_p <= 0.0f);
-    hipLaunchKernelGGL(sample_pick_kernel<T>, rows, block, 0, s, z, a, w);
+    hipLaunchKernelGGL(sample_pick_kernel<T>, rows, few, 0, s, z, a, w);
     VDB_HIP(hipGetLastError());
     if (!listed) {
         const int cuts = ceil_div(w.parts, PARTS_EACH);
         hipLaunchKernelGGL(sample_weigh_kernel<T>, dim3((unsigned)(n * cuts)), dim3(STREAM_NT), 0, s, z, a, w, cuts);
         VDB_HIP(hipGetLastError());
-        hipLaunchKernelGGL(sample_border_kernel<T>, rows, block, 0, s, z, a, w);
+        hipLaunchKernelGGL(sample_border_kernel<T>, rows, few, 0, s, z, a, w);
         VDB_HIP(hipGetLastError());
         if (a.d_top_p || a.top_p < 1.0f) {
             hipLaunchKernelGGL(sample_above_kernel<T>, dim3((unsigned)(n * cuts)), dim3(STREAM_NT), 0, s, z, a, w, cuts);
             VDB_HIP(hipGetLastError());
         }
     }
-    hipLaunchKernelGGL(sample_rest_kernel<T>, rows, block, 0, s, z, a, w);
+    hipLaunchKernelGGL(sample_rest_kernel<T>, rows, dim3(ROW_NT), 0, s, z, a, w);
     VDB_HIP(hipGetLastError());
     return VDB_OK;
 }
 
 template <class T> static int launch_sample(const T* z, int64_t n, const SampleArgs& a, void* d_work, hipStream_t s) {
     if (!by_whole_chip(a.vocab)) {
-        hipLaunchKernelGGL(sample_kernel<T>, dim3((unsigned)n), dim3(SAMPLE_NT), 0, s, z, a);
+        hipLaunchKernelGGL(sample_kernel<T>, dim3((unsigned)n), dim3(ROW_NT), 0, s, z, a);
         VDB_HIP(hipGetLastError());
         return VDB_OK;
     }
