@@ -29,8 +29,12 @@ template <class T> struct Piece {
             for (int i = 0; i < 4; ++i) raw[i] = __float_as_uint(x[i]);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                raw[i] = (uint32_t)__builtin_bit_cast(uint16_t, (T)x[2 * i]) | ((uint32_t)__builtin_bit_cast(uint16_t, (T)x[2 * i + 1]) << 16);
+            for (int i = 0; i < 4; ++i) {
+                typedef float f32x2 __attribute__((ext_vector_type(2)));
+                typedef T T2 __attribute__((ext_vector_type(2)));
+                const f32x2 pair = {x[2 * i], x[2 * i + 1]};
+                raw[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector(pair, T2));
+            }
         }
     }
 };
