@@ -435,7 +435,7 @@ int vdb_rows_lookup_dev(vdb_rows* h, const int64_t* d_rows, int64_t n, float sca
 /* Gradient of a lookup: table_grad[r] = scale * sum of grad[i] over the i with rows[i] == r, zero for rows nobody
  * looked up; with `accumulate` that is added to what table_grad holds and the other rows are not touched.  Row
  * numbers outside [0, n_rows) contribute nothing.  The positions are sorted by row number (stable) and every row is
- * summed in fp32 in an order that depends on the row numbers alone. */
+ * summed in fp32 in an order that depends on the row numbers alone.  n_rows and n below 2^30, dim at most 2^23. */
 int vdb_lookup_grad_workspace(int64_t n, int64_t n_rows, int dim, int64_t* bytes);
 int vdb_lookup_grad_dev(const void* d_grad, int grad_type, int64_t ld, const int64_t* d_rows, int64_t n, float scale,
                         void* d_table_grad, int table_type, int64_t n_rows, int dim, int64_t ld_table, int accumulate,

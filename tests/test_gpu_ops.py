@@ -257,6 +257,84 @@ def test_distill(ops, vocab, k, kind):
     assert torch.equal(here, grad2) and torch.equal(loss3, loss2)
 
 
+@pytest.mark.parametrize("n,vocab,kind", [(2, 8190, "bf16"), (700, 4099, "f32"), (2, 16391, "f16"), (600, 9001, "bf16"), (3, 33001, "bf16"), (520, 32771, "f16"),
+                                         (2, 65530, "f32"), (530, 65519, "bf16"), (1, 131057, "bf16"), (2, 131080, "f16"), (2, 300001, "bf16"), (1, 1000003, "f32")])
+def test_distill_long_rows(ops, n, vocab, kind):
+    """Rows around the sizes at which blocks change and rows are split, at every offset from a 16-byte border, both directions
+    against sums in 64 bits on the GPU.  Bounds as in test_distill, for exponents up to 40."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(n * vocab)
+    dtype, k = TYPES[kind], 11
+    room = torch.randn(n * (vocab + 1) + 16, device="cuda", generator=g).mul_(2.5).to(dtype)
+    z = room[3:3 + n * (vocab + 1)].view(n, vocab + 1)[:, :vocab]               # each row one element further from the border
+    t = torch.randn(n, k, device="cuda", generator=g) * 3
+    at = torch.randint(0, vocab, (n, k), device="cuda", generator=g)
+    w = torch.rand(n, device="cuda", generator=g) + 0.5
+    loss, stats = ops.distill(z, t, at)
+    grad = ops.distill_grad(z, t, at, stats, w)
+    loss2, grad2 = ops.distill_step(z, t, at, w)
+    p = torch.softmax(t.double(), 1)
+    logq = torch.log_softmax(z.double(), 1)
+    want = (p * (p.log() - logq.gather(1, at))).sum(1)
+    target = torch.zeros(n, vocab, device="cuda", dtype=torch.float64).scatter_add_(1, at, p)
+    e_logs = U * (8 * 40 + vocab / 256 + 64)
+    size = (p * (p.log() - logq.gather(1, at)).abs()).sum(1)
+    for got in (loss, loss2):
+        assert ((got.double() - want).abs() <= e_logs + U * 600 * size).all()
+    assert torch.equal(stats[:, 0], z.float().amax(1))
+    want = w.double()[:, None] * (logq.exp() - target)
+    tol = w.double()[:, None] * (logq.exp() * (U * 300 + e_logs) + target * U * 300)
+    half = torch.finfo(dtype).eps / 2
+    for got in (grad, grad2):
+        assert ((got.double() - want).abs() <= tol + torch.clamp(half * (want.abs() + tol), min=torch.finfo(dtype).smallest_normal * half)).all()
+    outside = room.clone()
+    assert torch.equal(ops.distill_step(z, t, at, w, out=z)[1], grad2)
+    inside = outside[3:3 + n * (vocab + 1)].view(n, vocab + 1)
+    inside[:, :vocab] = grad2
+    assert torch.equal(room.float(), outside.float())                           # in place, and nothing beside the rows
+
+
+def test_distill_many_rows(ops):
+    """More rows than one launch takes: the last ones are what they are by themselves."""
+    n, vocab, k = (1 << 21) + 7, 9, 3
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    z, t = torch.randn(n, vocab, device="cuda", generator=g).bfloat16(), torch.randn(n, k, device="cuda", generator=g)
+    at, w = torch.randint(0, vocab, (n, k), device="cuda", generator=g), torch.rand(n, device="cuda", generator=g)
+    loss, stats = ops.distill(z, t, at)
+    grad = ops.distill_grad(z, t, at, stats, w)
+    loss2, grad2 = ops.distill_step(z, t, at, w)
+    for lo, hi in ((0, 20), (n - 20, n)):
+        part = z[lo:hi], t[lo:hi], at[lo:hi]
+        one, its = ops.distill(*part)
+        assert torch.equal(loss[lo:hi], one) and torch.equal(stats[lo:hi], its)
+        assert torch.equal(grad[lo:hi], ops.distill_grad(*part, its, w[lo:hi]))
+        one, its = ops.distill_step(*part, w[lo:hi])
+        assert torch.equal(loss2[lo:hi], one) and torch.equal(grad2[lo:hi], its)
+
+
+def test_sample_many_rows(ops):
+    n, vocab = (1 << 21) + 7, 9
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    z, u = torch.randn(n, vocab, device="cuda", generator=g), torch.rand(n, device="cuda", generator=g)
+    top_p = torch.rand(n, device="cuda", generator=g)
+    row, logp = ops.sample(z, u, top_p=top_p)
+    for lo, hi in ((0, 20), (n - 20, n)):
+        one, its = ops.sample(z[lo:hi], u[lo:hi], top_p=top_p[lo:hi])
+        assert torch.equal(row[lo:hi], one) and torch.equal(logp[lo:hi], its)
+
+
+def test_lookup_many_rows(ops):
+    n, dim = (1 << 23) + 5, 1030
+    table = torch.randn(100, dim, device="cuda")
+    at = torch.arange(n, device="cuda") % 101                                   # 100: no row
+    out = ops.lookup(table, at, dtype=torch.bfloat16)
+    for lo, hi in ((0, 300), (n - 300, n)):
+        assert torch.equal(out[lo:hi], ops.lookup(table, at[lo:hi], dtype=torch.bfloat16))
+    assert torch.equal(out[n - 1], table[(n - 1) % 101].bfloat16())
+
+
 def test_distill_differences(ops):
     rng = rng_for("distill differences")
     z, t, at = distill_inputs(rng, 8, 40, 6, torch.float32)

@@ -28,7 +28,7 @@ __global__ void __launch_bounds__(256) lookup_kernel(const Ti* __restrict__ tabl
     const bool known = r >= 0 && r < n_rows;
     const Ti* src = table + (known ? r : 0) * ld;
     To* dst = out + i * ld_out;
-    for (int c = (threadIdx.x & (tpr - 1)) * N; c < dim; c += tpr * N) {
+    for (int64_t c = (threadIdx.x & (tpr - 1)) * N; c < dim; c += tpr * N) {
         float x[N];
         if (known) {
             load_values(src, c, dim, 0.0f, x);
@@ -473,9 +473,13 @@ int launch_lookup(const void* table, int table_type, int64_t n_rows, int dim, in
             typedef std::remove_pointer_t<decltype(ti)> Ti;
             typedef std::remove_pointer_t<decltype(to)> To;
             const int l = log_threads((dim + Piece<Ti>::N - 1) / Piece<Ti>::N);
-            hipLaunchKernelGGL((lookup_kernel<Ti, To>), dim3(ceil_div(n, 256 >> l)), dim3(256), 0, s, (const Ti*)table, n_rows, dim, ld, rows, n,
-                               scale, (To*)out, ld_out, l);
-            VDB_HIP(hipGetLastError());
+            const int64_t most = ((int64_t)1 << 31) >> l;             // a launch holds fewer than 2^32 threads
+            for (int64_t i = 0; i < n; i += most) {
+                const int64_t m = std::min(most, n - i);
+                hipLaunchKernelGGL((lookup_kernel<Ti, To>), dim3(ceil_div(m, 256 >> l)), dim3(256), 0, s, (const Ti*)table, n_rows, dim, ld, rows + i, m,
+                                   scale, (To*)out + i * ld_out, ld_out, l);
+                VDB_HIP(hipGetLastError());
+            }
             return VDB_OK;
         });
     });
@@ -610,7 +614,9 @@ int vdb_lookup_dev(const void* d_table, int table_type, int64_t n_rows, int dim,
 }
 
 static int check_grad_sizes(int64_t n, int64_t n_rows, int dim) {
-    VDB_REQUIRE(n >= 0 && n < LOOKUP_MAX && n_rows >= 0 && n_rows < LOOKUP_MAX && dim >= 1,
+    // what the grids of its launches hold
+    const int64_t most = (int64_t)1 << 30;
+    VDB_REQUIRE(n >= 0 && n < most && n_rows >= 0 && n_rows < most && dim >= 1 && dim <= 1 << 23,
                 "bad sizes for a lookup gradient: %lld rows into %lld, dimension %d", (long long)n, (long long)n_rows, dim);
     return VDB_OK;
 }

@@ -1317,13 +1317,11 @@ template <class T> static int launch_long_rows(const T* z, int64_t n, const Samp
 }
 
 template <class T> static int launch_sample(const T* z, int64_t n, const SampleArgs& a, void* d_work, hipStream_t s) {
-    if (!by_whole_chip(a.vocab)) {
-        hipLaunchKernelGGL(sample_kernel<T>, dim3((unsigned)n), dim3(ROW_NT), 0, s, z, a);
-        VDB_HIP(hipGetLastError());
-        return VDB_OK;
-    }
-    const SampleWork w = sample_work(d_work, std::min(n, SAMPLE_BATCH), a.vocab);
-    for (int64_t r = 0; r < n; r += SAMPLE_BATCH) {
+    const bool whole_chip = by_whole_chip(a.vocab);
+    const int64_t batch = whole_chip ? SAMPLE_BATCH : (int64_t)1 << 21;           // a launch holds fewer than 2^32 threads
+    const SampleWork w = whole_chip ? sample_work(d_work, std::min(n, batch), a.vocab) : SampleWork{};
+    for (int64_t r = 0; r < n; r += batch) {
+        const int64_t m = std::min(n - r, batch);
         SampleArgs b = a;
         b.uniform += r;
         if (b.d_temperature) b.d_temperature += r;
@@ -1333,7 +1331,11 @@ template <class T> static int launch_sample(const T* z, int64_t n, const SampleA
         if (b.mask) b.mask += r * b.mask_ld;
         b.out_row += r;
         if (b.out_logp) b.out_logp += r;
-        VDB_TRY(launch_long_rows(z + r * a.ld, std::min(n - r, SAMPLE_BATCH), b, w, s));
+        if (whole_chip) VDB_TRY(launch_long_rows(z + r * a.ld, m, b, w, s));
+        else {
+            hipLaunchKernelGGL(sample_kernel<T>, dim3((unsigned)m), dim3(ROW_NT), 0, s, z + r * a.ld, b);
+            VDB_HIP(hipGetLastError());
+        }
     }
     return VDB_OK;
 }
