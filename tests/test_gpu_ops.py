@@ -166,6 +166,25 @@ def test_lookup_grad_many_rows(ops):
     assert torch.equal(got.double(), want)
 
 
+@pytest.mark.parametrize("n", [15, 16, 17, 1000, 4096, 4097, 8192, 8193, 12287, 12288, 12289])
+@pytest.mark.parametrize("named", ["any", "two", "none", "one"])
+def test_lookup_grad_sizes(ops, n, named):
+    """Around the sizes at which the sort changes; rows named by nearly every position between rows that none names; rows that
+    end inside a piece.  Sums of whole numbers are exact (below 2^24)."""
+    rng = rng_for(n, named)
+    for n_rows, dim, kind in ((7, 19, "f32"), (130, 13, "bf16"), (5000, 21, "f16"), (60000, 3, "bf16")):
+        rows = {"any": rng.randint(-2, n_rows + 2, n), "two": rng.choice([3, 5], n), "none": np.full(n, -1), "one": np.full(n, n_rows - 1)}[named]
+        x = rng.randint(-3, 4, (n, dim)).astype(np.float32)
+        want = np.zeros((n_rows, dim))
+        known = (rows >= 0) & (rows < n_rows)
+        np.add.at(want, rows[known], x[known])
+        got = ops.lookup_grad(cuda(x, TYPES[kind]), cuda(rows.astype(np.int64)), n_rows, dtype=torch.float32)
+        assert (f64(got) == want).all()
+        out = torch.full((n_rows, dim + 2), 7.0, device="cuda")
+        ops.lookup_grad(cuda(x, TYPES[kind]), cuda(rows.astype(np.int64)), n_rows, out=out[:, :dim], accumulate=True)
+        assert (f64(out[:, :dim]) == want + 7).all() and bool((out[:, dim:] == 7).all())
+
+
 def test_lookup_grad_differences(ops):
     """The gradient of sum(w * lookup(table)) against the quotient of differences: linear, so the quotient is exact but for rounding."""
     rng = rng_for("differences")

@@ -123,14 +123,22 @@ __global__ void __launch_bounds__(64) sort_scan_kernel(int* __restrict__ hist, i
     if (threadIdx.x == 0) totals[blockIdx.x] = run;
 }
 
-// lanes of the wave whose digit equals this lane's (lanes without a key are in nobody's set)
-__device__ __forceinline__ unsigned long long same_digit(int d, int bits, bool have) {
+// Lanes of the wave whose digit equals this lane's (lanes without a key are in nobody's set).  All the bits that a digit can
+// have, unrolled: those above it are zero in every lane (a loop over its own bits takes a tenth longer).
+__device__ __forceinline__ unsigned long long same_digit(int d, bool have) {
     unsigned long long m = __ballot(have);
-    for (int b = 0; b < bits; ++b) {
-        const unsigned long long one = __ballot((d >> b) & 1);
-        m &= ((d >> b) & 1) ? one : ~one;
+    uint32_t lo = (uint32_t)m, hi = (uint32_t)(m >> 32);
+#pragma unroll
+    for (int b = 0; b < SORT_MAX_BITS; ++b) {
+        const int mine = (d << (31 - b)) >> 31;                      // all ones or none
+        const unsigned long long one = __ballot(mine != 0);
+        lo &= ~((uint32_t)one ^ (uint32_t)mine);
+        hi &= ~((uint32_t)(one >> 32) ^ (uint32_t)mine);
     }
-    return m;
+    return (unsigned long long)hi << 32 | lo;
+}
+__device__ __forceinline__ int lanes_below(unsigned long long m) {
+    return (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
 }
 
 __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __restrict__ rows, const int* __restrict__ keys,
@@ -181,9 +189,9 @@ __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __
         const bool have = i < hi;
         const int key = have ? key_of(rows, keys, i, n_rows) : 0;
         const int d = (key >> shift) & (bins - 1);
-        const unsigned long long m = same_digit(d, bits, have);
+        const unsigned long long m = same_digit(d, have);
         if (have) {
-            const int rank = __popcll(m & ((1ull << lane) - 1));
+            const int rank = lanes_below(m);
             const int base = mine[d];
             // the wave's LDS operations run in order: every lane has its base before the last of its set moves it on
             __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -195,87 +203,64 @@ __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __
     }
 }
 
-// Up to SORT_ONE_MAX positions: the whole sort in one block, the pairs in LDS between the digits.
-static constexpr int SORT_ONE_NT = 1024, SORT_ONE_WAVES = SORT_ONE_NT / 64, SORT_ONE_ITEMS = 8, SORT_ONE_MAX = SORT_ONE_NT * SORT_ONE_ITEMS;
+// Up to COUNT_MAX positions: each by itself counts those that come before it, smaller rows and equal ones of earlier positions, and
+// has its place, in one launch over the whole chip: n^2 comparisons of two instructions.  8192 positions take 10 us, where the
+// 6 launches of the digits take 26 and one block that sorted in LDS took 21; at 16384 both forms are even.
+// A block takes 16 * KEYS positions, KEYS a thread, and all the keys into LDS; its 16 threads of a share go through a 64th of them.
+static constexpr int COUNT_NT = 1024, COUNT_LANES = 16, COUNT_SHARES = COUNT_NT / COUNT_LANES, COUNT_MAX = 12288;
 
-__global__ void __launch_bounds__(SORT_ONE_NT) sort_one_kernel(const int64_t* __restrict__ rows, int n, int64_t n_rows, int bits, int passes,
-                                                               int* __restrict__ keys_out, int* __restrict__ pos_out, Fill fill) {
-    extern __shared__ int lds[];
-    if (blockIdx.x > 0) return fill_rows(fill, (int)blockIdx.x - 1, (int)gridDim.x - 1, SORT_ONE_NT);
-    const int bins = 1 << bits, room = (n + 63) & ~63;
-    int* skey = lds;
-    int* spos = lds + room;
-    int* start = lds + 2 * room;                       // [SORT_ONE_WAVES][bins]
-    __shared__ int wave_total[SORT_ONE_WAVES];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int per = ((n + SORT_ONE_WAVES - 1) / SORT_ONE_WAVES + 63) & ~63;
-    const int lo = min(wave * per, n), hi = min(lo + per, n);
-    int* mine = start + wave * bins;
-    int key[SORT_ONE_ITEMS], pos[SORT_ONE_ITEMS];
-    for (int pass = 0; pass < passes; ++pass) {
-        const int shift = pass * bits;
-        for (int d = tid; d < SORT_ONE_WAVES * bins; d += SORT_ONE_NT) start[d] = 0;
+template <int KEYS>
+__global__ void __launch_bounds__(COUNT_NT) sort_count_kernel(const int64_t* __restrict__ rows, int n, int64_t n_rows, int blocks, int* __restrict__ keys_out,
+                                                              int* __restrict__ pos_out, Fill fill) {
+    constexpr int TAKE = COUNT_LANES * KEYS, AHEAD = 4;
+    extern __shared__ __align__(16) int lds[];
+    if ((int)blockIdx.x >= blocks) return fill_rows(fill, (int)blockIdx.x - blocks, (int)gridDim.x - blocks, COUNT_NT);
+    __shared__ int before[COUNT_NT / 64][TAKE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, room = (n + 3) & ~3;
+    for (int i0 = tid; i0 < room; i0 += AHEAD * COUNT_NT) {
+        int64_t r[AHEAD];
 #pragma unroll
-        for (int q = 0; q < SORT_ONE_ITEMS; ++q) {
-            const int i = lo + q * 64 + lane;
-            key[q] = 0;
-            pos[q] = i;
-            if (i < hi) {
-                key[q] = pass == 0 ? key_of(rows, nullptr, i, n_rows) : skey[i];
-                if (pass > 0) pos[q] = spos[i];
-            }
+        for (int u = 0; u < AHEAD; ++u) r[u] = rows[min(i0 + u * COUNT_NT, n - 1)];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u * COUNT_NT;
+            if (i < room) lds[i] = i >= n ? 0x7fffffff : r[u] >= 0 && r[u] < n_rows ? (int)r[u] : (int)n_rows;
         }
-        __syncthreads();
-#pragma unroll
-        for (int q = 0; q < SORT_ONE_ITEMS; ++q)
-            if (lo + q * 64 + lane < hi) atomicAdd(&mine[(key[q] >> shift) & (bins - 1)], 1);
-        __syncthreads();
-        // one digit a thread: prefix over the digits, then over the waves of a digit
-        int total = 0;
-        if (tid < bins)
-            for (int w = 0; w < SORT_ONE_WAVES; ++w) total += start[w * bins + tid];
-        int inc = total;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int t = __shfl_up(inc, o);
-            if (lane >= o) inc += t;
-        }
-        if (lane == 63) wave_total[wave] = inc;
-        __syncthreads();
-        int at = inc - total;
-        for (int w = 0; w < wave; ++w) at += wave_total[w];
-        if (tid < bins)
-            for (int w = 0; w < SORT_ONE_WAVES; ++w) {
-                const int c = start[w * bins + tid];
-                start[w * bins + tid] = at;
-                at += c;
-            }
-        __syncthreads();
-        const bool last = pass + 1 == passes;
-#pragma unroll
-        for (int q = 0; q < SORT_ONE_ITEMS; ++q) {
-            const int i0 = lo + q * 64;
-            if (i0 >= hi) break;
-            const bool have = i0 + lane < hi;
-            const int d = (key[q] >> shift) & (bins - 1);
-            const unsigned long long m = same_digit(d, bits, have);
-            if (have) {
-                const int rank = __popcll(m & ((1ull << lane) - 1));
-                const int base = mine[d];
-                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-                if (rank == __popcll(m) - 1) mine[d] = base + rank + 1;
-                if (last) {
-                    keys_out[base + rank] = key[q];
-                    pos_out[base + rank] = pos[q];
-                } else {
-                    skey[base + rank] = key[q];
-                    spos[base + rank] = pos[q];
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        }
-        __syncthreads();
     }
+    __syncthreads();
+    const int first = (int)blockIdx.x * TAKE, share = tid / COUNT_LANES;
+    int key[KEYS], at[KEYS];
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) {
+        const int i = first + k * COUNT_LANES + (tid & (COUNT_LANES - 1));
+        key[k] = lds[min(i, n - 1)];
+        // equal ones among the block's own positions
+        const int j = first + share;
+        at[k] = share < TAKE && j < i && j < n && lds[j] == key[k];
+    }
+#pragma unroll 4
+    for (int q = share; q < room / 4; q += COUNT_SHARES) {
+        const int4 other = *(const int4*)(lds + 4 * q);
+        const int equal = 4 * q < first;
+#pragma unroll
+        for (int k = 0; k < KEYS; ++k) {
+            const int least = key[k] + equal;
+            at[k] += (other.x < least) + (other.y < least) + (other.z < least) + (other.w < least);
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < KEYS; ++k) {
+        at[k] += __shfl_xor(at[k], 16);
+        at[k] += __shfl_xor(at[k], 32);
+        if (lane < COUNT_LANES) before[wave][k * COUNT_LANES + lane] = at[k];
+    }
+    __syncthreads();
+    if (tid >= TAKE || first + tid >= n) return;
+    int place = 0;
+#pragma unroll
+    for (int w = 0; w < COUNT_NT / 64; ++w) place += before[w][tid];
+    keys_out[place] = lds[first + tid];
+    pos_out[place] = first + tid;
 }
 
 // ---------------------------------------------------------------- sums of the sorted rows
@@ -307,6 +292,9 @@ template <class To, int N> __device__ __forceinline__ void put_row(To* row, int 
     store_values<To, N>(row, c, dim, x);
 }
 
+// sums of a part of a row lie in whole pieces
+__host__ __device__ static inline int64_t part_pitch(int dim) { return ((int64_t)dim + 7) & ~7; }
+
 static constexpr int ZERO_ROWS = 64;
 
 // Blocks below zero_from: a group of 1 << log_tpr threads takes the chunk g of sorted positions; columns in slices of
@@ -329,7 +317,18 @@ __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ gra
             if ((threadIdx.x & 63) == 0) range[threadIdx.x >> 6] = at;
         }
         __syncthreads();
-        for (int64_t p = range[0] + threadIdx.x; p < range[1]; p += 256) named[keys[p] - r0] = 1;
+        if (range[1] - range[0] <= 8 * 256) {
+            for (int64_t p = range[0] + threadIdx.x; p < range[1]; p += 256) named[keys[p] - r0] = 1;
+        } else if (threadIdx.x < ZERO_ROWS) {            // rows named many times: each looks for itself (131072 positions of 10 rows: 161 us to go through)
+            const int64_t r = r0 + threadIdx.x;
+            uint32_t a = (uint32_t)range[0], b = (uint32_t)range[1];
+            while (a < b) {
+                const uint32_t mid = a + ((b - a) >> 1);
+                if (keys[mid] < r) a = mid + 1;
+                else b = mid;
+            }
+            named[threadIdx.x] = a < (uint32_t)range[1] && keys[a] == r;
+        }
         __syncthreads();
         constexpr int N = Piece<To>::N;
         float x[N];
@@ -348,39 +347,58 @@ __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ gra
     if (g >= chunks || c >= dim) return;
     const int64_t p0 = g * chunk, p1 = min(p0 + chunk, n);
     const int before = p0 > 0 ? keys[p0 - 1] : -1, behind = p1 < n ? keys[p1] : -1;
-    const bool whole = c + N <= dim;
+    const int64_t pitch = part_pitch(dim);
+    // a piece that ends behind the row is read from its last N values, what belongs to the thread before is dropped
+    const int skip = dim >= N ? max(c + N - dim, 0) : 0;
     float acc[N];
 #pragma unroll
     for (int e = 0; e < N; ++e) acc[e] = 0.0f;
+    int key[SEG_BATCH], from[SEG_BATCH];
+#pragma unroll
+    for (int q = 0; q < SEG_BATCH; ++q) key[q] = keys[min(p0 + q, n - 1)];
+#pragma unroll
+    for (int q = 0; q < SEG_BATCH; ++q) from[q] = pos[min(p0 + q, n - 1)];
     for (int64_t b = p0; b < p1; b += SEG_BATCH) {
-        int key[SEG_BATCH + 1];
+        if (key[0] >= n_rows) break;                     // the positions without a row come last
+        // No branch around the loads: where one joins, the compiler waits for loads that are still under way (1000000 x 64 fp32
+        // rows 220 us, so 149).
         Piece<Tg> x[SEG_BATCH];
+        int next[SEG_BATCH];
+        if (dim >= N) {
 #pragma unroll
-        for (int q = 0; q <= SEG_BATCH; ++q) key[q] = b + q < p1 ? keys[b + q] : -1;
+            for (int q = 0; q < SEG_BATCH; ++q) x[q] = load_piece(grad + (int64_t)from[q] * ld + (c - skip));
+        } else {
 #pragma unroll
-        for (int q = 0; q < SEG_BATCH; ++q) {
-            if (key[q] < 0 || key[q] >= n_rows) continue;
-            const Tg* src = grad + (int64_t)pos[b + q] * ld;
-            if (whole) x[q] = load_piece(src + c);
-            else {
+            for (int q = 0; q < SEG_BATCH; ++q) {
                 float v[N];
-                load_values(src, c, dim, 0.0f, v);
+                load_values(grad + (int64_t)from[q] * ld, c, dim, 0.0f, v);
                 x[q].set(v);
             }
         }
 #pragma unroll
+        for (int q = 0; q < SEG_BATCH; ++q) next[q] = keys[min(b + SEG_BATCH + q, n - 1)];
+#pragma unroll
+        for (int q = 0; q < SEG_BATCH; ++q) from[q] = pos[min(b + SEG_BATCH + q, n - 1)];
+        if (skip) {
+#pragma unroll
+            for (int q = 0; q < SEG_BATCH; ++q) x[q].drop_first(skip);
+        }
+#pragma unroll
         for (int q = 0; q < SEG_BATCH; ++q) {
             const int cur = key[q];
-            if (cur < 0 || cur >= n_rows) break;         // the positions without a row come last
+            if (b + q >= p1 || cur >= n_rows) break;
 #pragma unroll
             for (int e = 0; e < N; ++e) acc[e] += x[q].get(e);
-            if (key[q + 1] == cur) continue;
-            const bool open = b + q + 1 == p1 && behind == cur;
-            if (cur == before || open) store_values<float, N>(part + (g * 2 + (cur == before ? 0 : 1)) * dim, c, dim, acc);
+            const bool end = b + q + 1 == p1;
+            if (!end && (q + 1 < SEG_BATCH ? key[q + 1] : next[0]) == cur) continue;
+            const bool open = end && behind == cur;
+            if (cur == before || open) store_values<float, N>(part + (g * 2 + (cur == before ? 0 : 1)) * pitch, c, pitch, acc);
             else put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
 #pragma unroll
             for (int e = 0; e < N; ++e) acc[e] = 0.0f;
         }
+#pragma unroll
+        for (int q = 0; q < SEG_BATCH; ++q) key[q] = next[q];
     }
 }
 
@@ -391,12 +409,14 @@ __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ gra
 static constexpr int JOIN_NT = 1024, JOIN_WAVES = JOIN_NT / 64, JOIN_CHUNKS = 32;
 
 // parts [lo, hi) of the row that starts in chunk g: [g][1], then [g + 1][0], [g + 2][0], ...
-template <int N> __device__ __forceinline__ void add_parts(const float* part, int64_t g, int64_t lo, int64_t hi, int c, int dim, float* acc) {
+template <int N> __device__ __forceinline__ void add_parts(const float* part, int64_t pitch, int64_t g, int64_t lo, int64_t hi, int c, float* acc) {
     for (int64_t j = lo; j < hi; j += SEG_BATCH) {
         float x[SEG_BATCH][N];
 #pragma unroll
-        for (int q = 0; q < SEG_BATCH; ++q)
-            if (j + q < hi) load_values(part + ((g + j + q) * 2 + (j + q == 0 ? 1 : 0)) * dim, c, dim, 0.0f, x[q]);
+        for (int q = 0; q < SEG_BATCH; ++q) {
+            const int64_t k = min(j + q, hi - 1);
+            __builtin_memcpy(x[q], part + ((g + k) * 2 + (k == 0 ? 1 : 0)) * pitch + c, N * 4);
+        }
 #pragma unroll
         for (int q = 0; q < SEG_BATCH; ++q)
             if (j + q < hi) {
@@ -415,6 +435,7 @@ __global__ void __launch_bounds__(JOIN_NT) seg_join_kernel(const int* __restrict
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int c = blockIdx.y * 256 + lane * N;
     const bool active = c < dim;
+    const int64_t pitch = part_pitch(dim);
     bool starts = false, many = false;
     {
         const int64_t g = (int64_t)blockIdx.x * JOIN_CHUNKS + lane, p1 = (g + 1) * chunk;
@@ -435,7 +456,7 @@ __global__ void __launch_bounds__(JOIN_NT) seg_join_kernel(const int* __restrict
         for (int64_t p = (g + 1) * chunk; count < SEG_BATCH && p < n && keys[p] == cur; p += chunk) ++count;
         if (!active) continue;
         float acc[N] = {0.0f, 0.0f, 0.0f, 0.0f};
-        add_parts<N>(part, g, 0, count, c, dim, acc);
+        add_parts<N>(part, pitch, g, 0, count, c, acc);
         put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
     }
     for (unsigned long long todo = long_ones; todo; todo &= todo - 1) {
@@ -444,7 +465,7 @@ __global__ void __launch_bounds__(JOIN_NT) seg_join_kernel(const int* __restrict
         const int64_t end = lower_bound_wave(keys, n, (int64_t)cur + 1), count = (end - 1) / chunk - g + 1;
         const int64_t per = (count + JOIN_WAVES - 1) / JOIN_WAVES, lo = wave * per, hi = lo + per < count ? lo + per : count;
         float acc[N] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (active) add_parts<N>(part, g, lo, hi, c, dim, acc);
+        if (active) add_parts<N>(part, pitch, g, lo, hi, c, acc);
         __syncthreads();
 #pragma unroll
         for (int e = 0; e < N; ++e) sums[wave][lane * N + e] = acc[e];
@@ -500,7 +521,7 @@ static int seg_chunk(int64_t n, int dim) {
     return 8;
 }
 // Whether the whole table is zeroed beside the sort, and the named rows written over it: where those are few (10240 x 384
-// into 100000 rows: 22 us of zeros behind 30 us of sorting), else the sums' launch writes zeros to the other rows alone.
+// into 100000 rows: 28 us with the sort, which takes 12 by itself), else the sums' launch writes zeros to the other rows alone.
 static bool fill_first(int64_t n, int64_t n_rows) { return n > 0 && n <= n_rows / 4; }
 static GradWork grad_work(void* base, int64_t n, int64_t n_rows, int dim) {
     const SortPlan p = sort_plan(n, n_rows);
@@ -513,12 +534,12 @@ static GradWork grad_work(void* base, int64_t n, int64_t n_rows, int dim) {
     };
     for (int i = 0; i < 2; ++i) w.keys[i] = (int*)take(n * 4);
     for (int i = 0; i < 2; ++i) w.pos[i] = (int*)take(n * 4);
-    if (n > SORT_ONE_MAX) {
+    if (n > COUNT_MAX) {
         w.hist = (int*)take(((int64_t)p.blocks << p.bits) * 4);
         w.totals = (int*)take(((int64_t)1 << p.bits) * 4);
     }
     const int chunk = seg_chunk(n, dim);
-    w.part = (float*)take((n + chunk - 1) / chunk * 2 * dim * 4);
+    w.part = (float*)take((n + chunk - 1) / chunk * 2 * part_pitch(dim) * 4);
     w.bytes = at - (char*)base;
     return w;
 }
@@ -536,13 +557,15 @@ static int launch_sort(const int64_t* rows, int64_t n, int64_t n_rows, const Gra
         return (int)std::min<int64_t>(((hi - lo) * fill.units * 2 + 32767) / 32768, (int64_t)ctx().num_cus * 2048 / threads);
     };
     const int64_t fill_end = fill.out ? n_rows : 0;
-    if (n <= SORT_ONE_MAX) {
-        const size_t lds = (2 * (size_t)round_up64(n, 64) + (size_t)SORT_ONE_WAVES * bins) * 4;
-        VDB_TRY(raise_dynamic_lds((const void*)sort_one_kernel, (2 * (size_t)SORT_ONE_MAX + ((size_t)SORT_ONE_WAVES << SORT_MAX_BITS)) * 4));
-        const int extra = fill_blocks(0, fill_end, SORT_ONE_NT);
-        hipLaunchKernelGGL(sort_one_kernel, dim3(1 + extra), dim3(SORT_ONE_NT), lds, s, rows, (int)n, n_rows, p.bits, p.passes, const_cast<int*>(*keys),
-                           const_cast<int*>(*pos), fill);
+    if (n <= COUNT_MAX) {
+        const int per = std::min(std::max(ceil_div(n, COUNT_LANES * ctx().num_cus), 1), 3), blocks = ceil_div(n, COUNT_LANES * per);
+        const int extra = fill_blocks(0, fill_end, COUNT_NT);
+        auto kernel = per == 1 ? sort_count_kernel<1> : per == 2 ? sort_count_kernel<2> : sort_count_kernel<3>;
+        VDB_TRY(raise_dynamic_lds((const void*)kernel, COUNT_MAX * 4));
+        hipLaunchKernelGGL(kernel, dim3(blocks + extra), dim3(COUNT_NT), (size_t)round_up64(n, 4) * 4, s, rows, (int)n, n_rows, blocks, w.keys[0], w.pos[0], fill);
         VDB_HIP(hipGetLastError());
+        *keys = w.keys[0];
+        *pos = w.pos[0];
         return VDB_OK;
     }
     const int shares = 2 * p.passes;

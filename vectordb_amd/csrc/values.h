@@ -23,6 +23,13 @@ template <class T> struct Piece {
         else if constexpr (__is_same(T, bf16_t)) return __uint_as_float((i & 1) ? (raw[i >> 1] & 0xffff0000u) : (raw[i >> 1] << 16));
         else return (float)__builtin_bit_cast(f16_t, (uint16_t)((i & 1) ? (raw[i >> 1] >> 16) : (raw[i >> 1] & 0xffffu)));
     }
+    // the first n elements away, the others to the front
+    __device__ __forceinline__ void drop_first(int n) {
+        const int bytes = n * (int)sizeof(T);
+        if (bytes & 8) raw = u32x4{raw[2], raw[3], 0u, 0u};
+        if (bytes & 4) raw = u32x4{raw[1], raw[2], raw[3], 0u};
+        if (bytes & 2) raw = u32x4{raw[0] >> 16 | raw[1] << 16, raw[1] >> 16 | raw[2] << 16, raw[2] >> 16 | raw[3] << 16, raw[3] >> 16};
+    }
     __device__ __forceinline__ void set(const float* x) {
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
