@@ -285,9 +285,16 @@ template <class To, int N> __device__ __forceinline__ void put_row(To* row, int 
 #pragma unroll
     for (int e = 0; e < N; ++e) x[e] = scale * acc[e];
     if (accumulate) {
+        if (c + N <= dim) {
+            To old[N];
+            __builtin_memcpy(old, row + c, sizeof(old));
 #pragma unroll
-        for (int e = 0; e < N; ++e)
-            if (c + e < dim) x[e] = (float)row[c + e] + x[e];
+            for (int e = 0; e < N; ++e) x[e] = (float)old[e] + x[e];
+        } else {
+#pragma unroll
+            for (int e = 0; e < N; ++e)
+                if (c + e < dim) x[e] = (float)row[c + e] + x[e];
+        }
     }
     store_values<To, N>(row, c, dim, x);
 }
