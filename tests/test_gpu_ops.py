@@ -495,6 +495,56 @@ def test_sample_ties(ops, top_k, top_p, min_p):
         sample_check(ops, cuda(z, TYPES[kind]), u, allowed, top_k=top_k, top_p=top_p, min_p=min_p, temperature=0.5)
 
 
+@pytest.mark.parametrize("top_k,top_p,min_p", [(0, 1.0, 0.0), (5, 1.0, 0.0), (2500, 0.9, 0.0), (30000, 1.0, 0.0), (0, 0.25, 0.0), (0, 0.7, 0.0), (0, 1.0, 0.4), (0, 0.95, 0.9)])
+def test_sample_ties_long(ops, top_k, top_p, min_p):
+    """The same in rows that the whole chip goes through: thousands of equal scores at a border, rows of one value, filters
+    that leave single scores, whole stretches or nothing."""
+    rng = rng_for("ties long", top_k, top_p)
+    n, vocab = 12, 40_009
+    z = rng.randint(-2, 3, (n, vocab)).astype(np.float32)
+    z[:3] = 1.0
+    z[3] = -0.0
+    z[3, ::3] = 0.0
+    z[4, 20_000:] = np.finfo(np.float32).min
+    z[5] = -np.inf
+    z[5, [7, 40_008]] = 0.0
+    z[6, ::2] = math.nan
+    u = rng.rand(n).astype(np.float32)
+    u[:3] = [0.0, 0.5, 1 - 2.0 ** -24]
+    allowed = rng.rand(n, vocab) < 0.7
+    allowed[7] = False
+    allowed[8] = False
+    allowed[8, 33_333] = True
+    allowed[9, :39_000] = False
+    for kind in ("f32", "f16"):
+        with np.errstate(over="ignore"):
+            scores = cuda(z, TYPES[kind])
+        sample_check(ops, scores, u, top_k=top_k, top_p=top_p, min_p=min_p)
+        sample_check(ops, scores, u, allowed, top_k=top_k, top_p=top_p, min_p=min_p, temperature=0.5)
+    sample_check(ops, cuda(-z), u, allowed[10], distances=True, top_k=top_k, top_p=top_p, min_p=min_p)
+
+
+def test_sample_long_batches(ops):
+    """More long rows than are worked on at a time, each with settings and a filter of its own: what they are by themselves."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(8)
+    n, vocab = 2050, 33_000
+    r = lambda *s: torch.rand(*s, device="cuda", generator=g)               # noqa: E731
+    z, u = torch.randn(n, vocab, device="cuda", generator=g).bfloat16() * 2, r(n)
+    tau, top_p, min_p = r(n) * 2, r(n) * 1.2, (r(n) - 0.5).clamp(min=0)
+    top_k = torch.randint(0, 4, (n,), device="cuda", generator=g, dtype=torch.int32) * 60
+    words = torch.randint(-2 ** 31, 2 ** 31, (n, (vocab + 31) // 32), device="cuda", generator=g).int()
+    row, logp = ops.sample(z, u, tau, top_k, top_p, min_p, words)
+    for i in (0, 1, 1023, 1024, 1025, 2047, 2048, 2049):
+        s = slice(i, i + 1)
+        one = ops.sample(z[s], u[s], tau[s], top_k[s], top_p[s], min_p[s], words[s])
+        assert torch.equal(row[s], one[0]) and torch.equal(logp[s], one[1]), i
+        bits = words[i].cpu().numpy().view(np.uint32)
+        allowed = np.unpackbits(bits.view(np.uint8), bitorder="little")[:vocab].astype(bool)
+        want, wlog = R.sample_row(f64(z[i]), float(u[i]), float(tau[i]), int(top_k[i]), float(top_p[i]), float(min_p[i]), allowed)
+        assert int(row[i]) == want and abs(float(logp[i]) - wlog) <= U * abs(wlog) + 1e-10, i
+
+
 def test_sample_odd_rows(ops):
     rng = rng_for("odd sample")
     inf = math.inf
