@@ -418,8 +418,9 @@ int vdb_topk_merge_keyed_strided_dev(const float* d_dist, const int64_t* d_key, 
  *
  * All take DEVICE pointers and the stream to enqueue on (NULL = the null stream), never synchronise and never
  * allocate, so they can be captured into a graph; what they need beside inputs and outputs is the caller's `d_work`
- * of at least the bytes that the *_workspace function names, which holds nothing between calls (two calls that may
- * overlap take two).  Values are fp32, bf16 or fp16 (vdb_value_type); products and sums are taken in 32 bits or
+ * of at least the bytes that the *_workspace function names (after vdb_init), at a multiple of 16 bytes, which holds
+ * nothing between calls (two calls that may overlap take two).  Outputs overlap neither inputs nor each other but
+ * where it is said.  Values are fp32, bf16 or fp16 (vdb_value_type); products and sums are taken in 32 bits or
  * more and rounded once.  Rows of a matrix are contiguous and `ld` elements apart (0 for an input = one row for
  * all); no alignment beyond the type's own is asked for.  Results do not depend on timing: equal inputs give equal
  * bits.  n = 0 is allowed and does nothing. */

@@ -57,6 +57,19 @@ def test_c_abi_refuses(fn, base, change, text):
     refused(fn, *{**base, **change}.values(), text=text)
 
 
+ODD = C.c_void_p(4096 + 8)
+
+
+@pytest.mark.parametrize("fn,base,change,text", [
+    ("vdb_lookup_grad_dev", GRAD, dict(work=ODD), "16 bytes"), ("vdb_distill_dev", DISTILL, dict(work=ODD), "16 bytes"),
+    ("vdb_distill_step_dev", STEP, dict(work=ODD), "16 bytes"), ("vdb_sample_dev", SAMPLE, dict(work=ODD), "16 bytes"),
+    ("vdb_lookup_grad_dev", GRAD, dict(n=1 << 30), "bad sizes"), ("vdb_lookup_grad_dev", GRAD, dict(n_rows=1 << 30), "bad sizes"),
+    ("vdb_lookup_grad_dev", GRAD, dict(dim=(1 << 23) + 1, ldo=1 << 24), "bad sizes"),
+])
+def test_limits(fn, base, change, text):
+    refused(fn, *{**base, **change}.values(), text=text)
+
+
 def test_workspace_sizes():
     lib = _native.load()
     b = C.c_int64(-1)

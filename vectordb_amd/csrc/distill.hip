@@ -610,6 +610,7 @@ static int check_work(int64_t n, int64_t vocab, const void* d_work, int64_t work
     VDB_TRY(vdb_distill_workspace(n, vocab, &need));
     VDB_REQUIRE(work_bytes >= need && (d_work || need == 0), "the workspace of %lld bytes is too small for this distillation (%lld needed)",
                 (long long)work_bytes, (long long)need);
+    VDB_REQUIRE(aligned_work(d_work), "a workspace begins at a multiple of 16 bytes");
     return VDB_OK;
 }
 

@@ -668,6 +668,7 @@ int vdb_lookup_grad_dev(const void* d_grad, int grad_type, int64_t ld, const int
     const int64_t need = grad_work(nullptr, n, n_rows, dim).bytes;
     VDB_REQUIRE(work_bytes >= need && (d_work || need == 0), "the workspace of %lld bytes is too small for this lookup gradient (%lld needed)",
                 (long long)work_bytes, (long long)need);
+    VDB_REQUIRE(aligned_work(d_work), "a workspace begins at a multiple of 16 bytes");
     if (n_rows == 0 || (n == 0 && accumulate)) return VDB_OK;
     VDB_TRY(ensure_init());
     (void)hipSetDevice(ctx().device);

@@ -1365,6 +1365,7 @@ int vdb_sample_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int
     VDB_REQUIRE(n == 0 || (d_scores && d_uniform && d_out_row), "null pointer in sampling from %lld rows", (long long)n);
     VDB_REQUIRE(work_bytes >= need && (d_work || need == 0), "the workspace of %lld bytes is too small for this sampling (%lld needed)",
                 (long long)work_bytes, (long long)need);
+    VDB_REQUIRE(aligned_work(d_work), "a workspace begins at a multiple of 16 bytes");
     if (n == 0) return VDB_OK;
     VDB_TRY(ensure_init());
     (void)hipSetDevice(ctx().device);

@@ -82,6 +82,8 @@ template <class T, int N> __device__ __forceinline__ void store_values(T* row, i
 // host side: vdb_value_type codes to template arguments
 static inline bool valid_type(int type) { return type == VDB_VALUE_F32 || type == VDB_VALUE_BF16 || type == VDB_VALUE_F16; }
 
+static inline bool aligned_work(const void* work) { return ((uintptr_t)work & 15) == 0; }
+
 template <class F> static int with_type(int type, F&& f) {
     if (type == VDB_VALUE_F32) return f((float*)nullptr);
     if (type == VDB_VALUE_BF16) return f((bf16_t*)nullptr);

@@ -14,7 +14,8 @@ row) slots with row -1 where there is nothing; the filters of ``sample`` are the
 Every function enqueues on the current torch stream and returns without waiting; inputs made on another stream have to
 be ordered by the caller, as for any torch operation.  Nothing is allocated but the outputs (or none, with ``out=``) and a
 workspace from torch's allocator, so the calls can be captured into a graph.  Autograd does not see them: gradients are
-the functions named ``*_grad``, which a ``torch.autograd.Function`` can call.  Values are float32, bfloat16 or float16, sums
+the functions named ``*_grad``, which a ``torch.autograd.Function`` can call.  An ``out`` shares no memory with the inputs but
+where it is said.  Values are float32, bfloat16 or float16, sums
 are taken in 32 bits or more, and equal inputs give equal bits.  Arguments that do not fit raise ``ValueError``.
 """
 
