@@ -593,7 +593,7 @@ static int enter() {
 
 using namespace vdb;
 
-// the stats of a step in two passes, and the parts of long rows
+// the stats of a step in two passes, and the parts of long rows, which are no shorter
 static int64_t distill_stats_bytes(int64_t n) { return round_up64(n * 2 * (int64_t)sizeof(float), 256); }
 
 int vdb_distill_workspace(int64_t n, int64_t vocab, int64_t* bytes) {
@@ -602,7 +602,7 @@ int vdb_distill_workspace(int64_t n, int64_t vocab, int64_t* bytes) {
     // whatever the type: rows of fp32 have the most pieces
     int64_t part;
     const int parts = loss_parts(n, vocab, 4, &part);
-    *bytes = distill_stats_bytes(n) + (parts > 1 ? n * parts * (int64_t)sizeof(MaxSum) : 0);
+    *bytes = (step_shape(n, vocab, 4).nt ? 0 : distill_stats_bytes(n)) + (parts > 1 ? n * parts * (int64_t)sizeof(MaxSum) : 0);
     return VDB_OK;
 }
 static int check_work(int64_t n, int64_t vocab, const void* d_work, int64_t work_bytes) {
