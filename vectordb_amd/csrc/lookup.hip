@@ -412,7 +412,9 @@ __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ gra
 // The rows that cross chunks.  A block looks at JOIN_CHUNKS chunks and takes 256 columns (blockIdx.y): a row that starts
 // in one of them and goes on has its parts, here and in the following chunks, added in order; up to SEG_BATCH parts by one
 // wave (the block's waves take such rows side by side), more by all waves, a contiguous run of parts each.  What takes the
-// time is the latency of the parts' loads (2 us a batch: other XCDs wrote them), so as many as possible are in flight.
+// time is the latency of the parts' loads (2 us a batch: other XCDs wrote them), so as many as possible are in flight, and
+// a row's chunks are counted by a wave's probes at once (one after the other: 26 us, so 23, for 131072 rows of 2048 values
+// named as often as words are).
 static constexpr int JOIN_NT = 1024, JOIN_WAVES = JOIN_NT / 64, JOIN_CHUNKS = 32;
 
 // parts [lo, hi) of the row that starts in chunk g: [g][1], then [g + 1][0], [g + 2][0], ...
@@ -443,34 +445,42 @@ __global__ void __launch_bounds__(JOIN_NT) seg_join_kernel(const int* __restrict
     const int c = blockIdx.y * 256 + lane * N;
     const bool active = c < dim;
     const int64_t pitch = part_pitch(dim);
-    bool starts = false, many = false;
+    const int64_t first = (int64_t)blockIdx.x * JOIN_CHUNKS;
+    // key at the start of chunk j
+    auto border = [&](int64_t j) { return keys[min(j * chunk, n - 1)]; };
+    int row;                             // of the last position of chunk first + lane
+    bool starts, many;
     {
-        const int64_t g = (int64_t)blockIdx.x * JOIN_CHUNKS + lane, p1 = (g + 1) * chunk;
-        if (lane < JOIN_CHUNKS && g + 1 < chunks) {
-            const int cur = keys[p1 - 1];
-            starts = cur < n_rows && keys[p1] == cur && !(g > 0 && keys[p1 - chunk - 1] == cur);
-            const int64_t far = (g + SEG_BATCH) * chunk;            // the first position of part number SEG_BATCH
-            many = starts && far < n && keys[far] == cur;
-        }
+        const int64_t g = first + min(lane, JOIN_CHUNKS - 1), p1 = min((g + 1) * chunk, n);
+        row = keys[p1 - 1];
+        const int next = border(g + 1), prev = keys[max(p1 - chunk - 1, (int64_t)0)], far = border(g + SEG_BATCH);
+        starts = lane < JOIN_CHUNKS && g + 1 < chunks && row < n_rows && next == row && !(g > 0 && prev == row);
+        many = starts && g + SEG_BATCH < chunks && far == row;
     }
     const unsigned long long few = __ballot(starts && !many), long_ones = __ballot(many);
     int turn = 0;
     for (unsigned long long todo = few; todo; todo &= todo - 1, ++turn) {
         if (turn % JOIN_WAVES != wave) continue;
-        const int64_t g = (int64_t)blockIdx.x * JOIN_CHUNKS + __builtin_ctzll(todo);
-        const int cur = keys[(g + 1) * chunk - 1];
-        int count = 1;
-        for (int64_t p = (g + 1) * chunk; count < SEG_BATCH && p < n && keys[p] == cur; p += chunk) ++count;
+        const int at = __builtin_ctzll(todo), cur = __shfl(row, at);
+        const int64_t g = first + at;
+        const int count = __builtin_ctzll(~__ballot(lane == 0 || (lane < SEG_BATCH && g + lane < chunks && border(g + lane) == cur)));
         if (!active) continue;
         float acc[N] = {0.0f, 0.0f, 0.0f, 0.0f};
         add_parts<N>(part, pitch, g, 0, count, c, acc);
         put_row<To, N>(out + (int64_t)cur * ld_out, c, dim, scale, acc, accumulate);
     }
     for (unsigned long long todo = long_ones; todo; todo &= todo - 1) {
-        const int64_t g = (int64_t)blockIdx.x * JOIN_CHUNKS + __builtin_ctzll(todo);
-        const int cur = keys[(g + 1) * chunk - 1];
-        const int64_t end = lower_bound_wave(keys, n, (int64_t)cur + 1), count = (end - 1) / chunk - g + 1;
-        const int64_t per = (count + JOIN_WAVES - 1) / JOIN_WAVES, lo = wave * per, hi = lo + per < count ? lo + per : count;
+        const int at = __builtin_ctzll(todo), cur = __shfl(row, at);
+        const int64_t g = first + at;
+        // the chunks from g on that begin with the row (g itself counts): 64 probes a step
+        uint32_t count = SEG_BATCH, most = (uint32_t)(chunks - g);             // it lies in [count, most]
+        while (count < most) {
+            const uint32_t step = (most - count + 63) >> 6, probe = count + step * (lane + 1) - 1;
+            const uint32_t same = (uint32_t)__popcll(__ballot(probe < most && border(g + probe) == cur));
+            most = min(most, count + step * (same + 1) - 1);
+            count += step * same;
+        }
+        const uint32_t per = (count + JOIN_WAVES - 1) / JOIN_WAVES, lo = min(wave * per, count), hi = min(lo + per, count);
         float acc[N] = {0.0f, 0.0f, 0.0f, 0.0f};
         if (active) add_parts<N>(part, pitch, g, lo, hi, c, acc);
         __syncthreads();
