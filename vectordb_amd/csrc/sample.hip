@@ -1286,7 +1286,7 @@ template <class T> __global__ void __launch_bounds__(ROW_NT) sample_rest_kernel(
 // block each and by the whole chip: one row with top-k 50 12 and 13 us, top-p 0.9 44 and 30 us; 256 rows with settings of
 // every kind 49 and 60 us, 1024 rows 106 and 100 us.
 static bool by_whole_chip(int64_t vocab) { return vocab > 32768; }
-static const int64_t SAMPLE_BATCH = 1024;           // rows at a time by the whole chip: bounds the workspace (56 MB at 131072 scores)
+static const int64_t SAMPLE_BATCH = 1024;           // rows at a time by the whole chip: bounds the workspace (59 MB at 131072 scores)
 
 template <class T> static int launch_long_rows(const T* z, int64_t n, const SampleArgs& a, const SampleWork& w, hipStream_t s) {
     const dim3 rows((unsigned)n), few(FEW_NT);
