@@ -185,6 +185,41 @@ def test_lookup_grad_sizes(ops, n, named):
         assert (f64(out[:, :dim]) == want + 7).all() and bool((out[:, dim:] == 7).all())
 
 
+@pytest.mark.parametrize("kind", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("n_rows,dim,n", [(1, 1, 0), (3, 1, 1), (5, 3, 1), (700, 33, 100), (100000, 7, 20), (90000, 5, 15000), (300, 129, 250)])
+def test_lookup_grad_zeros(ops, kind, n_rows, dim, n):
+    """Zeros over rows that lie back to back, at every offset from a 16-byte border, and over rows apart: all of them, nothing beside."""
+    rng = rng_for("zeros", kind, n_rows)
+    rows = rng.randint(0, n_rows, n)
+    x = rng.randint(-3, 4, (n, dim)).astype(np.float32)
+    want = np.zeros((n_rows, dim))
+    np.add.at(want, rows, x)
+    for off in range(9):
+        room = torch.full((n_rows * dim + 20,), 7.0, device="cuda", dtype=TYPES[kind])
+        out = room[off:off + n_rows * dim].view(n_rows, dim)
+        ops.lookup_grad(cuda(x, TYPES[kind]), cuda(rows.astype(np.int64)), n_rows, out=out)
+        assert (f64(out) == want).all() and bool((room[:off] == 7).all()) and bool((room[off + n_rows * dim:] == 7).all()), off
+    room = torch.full((n_rows, dim + 3), 7.0, device="cuda", dtype=TYPES[kind])
+    ops.lookup_grad(cuda(x, TYPES[kind]), cuda(rows.astype(np.int64)), n_rows, out=room[:, :dim])
+    assert (f64(room[:, :dim]) == want).all() and bool((room[:, dim:] == 7).all())
+
+
+@pytest.mark.parametrize("dim", [1, 2, 3, 4, 7, 8, 9, 255, 1023, 1024, 1025, 2047, 4099, 8193])
+@pytest.mark.parametrize("tin,tout", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+def test_lookup_dimensions(ops, dim, tin, tout):
+    """Rows of one piece to many, few rows and as many as change how a block takes them; nothing is written beside."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(dim)
+    table = torch.randn(40, dim + 1, device="cuda", generator=g).to(TYPES[tin])[:, :dim]
+    for n in (1, 9, 3000, 4_000_000 // dim):
+        at = torch.randint(-1, 41, (n,), device="cuda", generator=g)
+        room = torch.full((n, dim + 1), 7.0, device="cuda", dtype=TYPES[tout])
+        ops.lookup(table, at, scale=0.5, out=room[:, :dim])
+        want = (table.float()[at.clamp(0, 39)] * 0.5).to(TYPES[tout])
+        want[(at < 0) | (at > 39)] = 0
+        assert torch.equal(room[:, :dim], want) and bool((room[:, dim:] == 7).all()), n
+
+
 def test_lookup_grad_differences(ops):
     """The gradient of sum(w * lookup(table)) against the quotient of differences: linear, so the quotient is exact but for rounding."""
     rng = rng_for("differences")

@@ -1,13 +1,13 @@
 // Rows of a table by number (vdb_lookup_dev) and the gradient of that table (vdb_lookup_grad_dev).
 //
-// lookup: out[i] = scale * table[rows[i]].  A copy of n rows; what bounds it is HBM traffic, n * dim values read and
-// written.  A group of threads (a power of two, up to a block) takes a row in 16-byte pieces.
+// lookup: out[i] = scale * table[rows[i]].  A copy of n rows in 16-byte pieces, four a thread; what bounds it is HBM traffic,
+// n * dim values written and as many read (from cache where rows repeat): 131072 x 2048 bf16 185 us, 5.8 TB/s.
 //
-// gradient: table_grad[r] = scale * sum over {i : rows[i] == r} of grad[i].  The positions i are sorted by row number
-// with a stable radix sort, so the members of a row lie side by side in ascending i; the sorted positions are cut into
-// chunks of SEG_CHUNK, a group of threads adds the rows of a chunk in order, and a row that crosses chunks has its
-// parts added in chunk order by a second launch.  No atomics on values: the order of every sum is fixed by the row
-// numbers.  Bound: grad read once, table_grad written once (rows without members as zeros).
+// gradient: table_grad[r] = scale * sum over {i : rows[i] == r} of grad[i].  The positions i are sorted by row number, stable,
+// so the members of a row lie side by side in ascending i; the sorted positions are cut into chunks of 8 to 64, a group of
+// threads adds the rows of a chunk in order, and a row that crosses chunks has its parts added in chunk order by a
+// second launch.  No atomics on values: the order of every sum is fixed by the row numbers.  Bound: grad read once,
+// table_grad written once (rows without members as zeros): 131072 x 2048 bf16 into 131072 fp32 rows 387 us, 4.2 TB/s.
 #include "vdb_internal.h"
 #include "values.h"
 
@@ -16,29 +16,52 @@
 namespace vdb {
 
 // ---------------------------------------------------------------- lookup
+// A block takes `take` rows, `pieces` pieces of 16 bytes each, AHEAD of them a thread at a time.  inverse = ceil(2^32 / pieces):
+// the row of piece x is the upper half of x * inverse (exact below 2^16), x itself lies in the only row otherwise.
+static constexpr int LOOKUP_NT = 256, LOOKUP_AHEAD = 4;
 template <class Ti, class To>
-__global__ void __launch_bounds__(256) lookup_kernel(const Ti* __restrict__ table, int64_t n_rows, int dim, int64_t ld,
-                                                     const int64_t* __restrict__ rows, int64_t n, float scale, To* __restrict__ out,
-                                                     int64_t ld_out, int log_tpr) {
+__global__ void __launch_bounds__(LOOKUP_NT) lookup_kernel(const Ti* __restrict__ table, int64_t n_rows, int dim, int64_t ld,
+                                                           const int64_t* __restrict__ rows, int64_t n, float scale, To* __restrict__ out,
+                                                           int64_t ld_out, int take, uint32_t pieces, uint32_t inverse) {
     constexpr int N = Piece<Ti>::N;
-    const int tpr = 1 << log_tpr;
-    const int64_t i = (int64_t)blockIdx.x * (256 >> log_tpr) + (threadIdx.x >> log_tpr);
-    if (i >= n) return;
-    const int64_t r = rows[i];
-    const bool known = r >= 0 && r < n_rows;
-    const Ti* src = table + (known ? r : 0) * ld;
-    To* dst = out + i * ld_out;
-    for (int64_t c = (threadIdx.x & (tpr - 1)) * N; c < dim; c += tpr * N) {
-        float x[N];
-        if (known) {
-            load_values(src, c, dim, 0.0f, x);
+    const int64_t first = (int64_t)blockIdx.x * take;
+    const uint32_t mine = (uint32_t)min((int64_t)take, n - first), all = mine * pieces;
+    for (uint32_t x0 = threadIdx.x; x0 < all; x0 += LOOKUP_AHEAD * LOOKUP_NT) {
+        int64_t r[LOOKUP_AHEAD];
+        uint32_t i[LOOKUP_AHEAD], c[LOOKUP_AHEAD];
+        Piece<Ti> v[LOOKUP_AHEAD];
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[e] *= scale;
+        for (int u = 0; u < LOOKUP_AHEAD; ++u) {
+            const uint32_t x = min(x0 + u * LOOKUP_NT, all - 1);
+            i[u] = pieces == 1 ? x : take == 1 ? 0 : __umulhi(x, inverse);
+            c[u] = (x - i[u] * pieces) * N;
+            r[u] = rows[first + i[u]];
+        }
+        if (dim >= N) {
+            // a piece that would end behind the row is the row's last N values: what two threads write there is the same
+#pragma unroll
+            for (int u = 0; u < LOOKUP_AHEAD; ++u) {
+                c[u] = min(c[u], (uint32_t)(dim - N));
+                v[u] = Piece<Ti>{};
+                if (r[u] >= 0 && r[u] < n_rows) v[u] = load_piece(table + r[u] * ld + c[u]);
+            }
         } else {
 #pragma unroll
-            for (int e = 0; e < N; ++e) x[e] = 0.0f;
+            for (int u = 0; u < LOOKUP_AHEAD; ++u) {
+                float y[N];
+                load_values(table + r[u] * ld, 0, r[u] >= 0 && r[u] < n_rows ? dim : 0, 0.0f, y);
+                v[u].set(y);
+            }
         }
-        store_values<To, N>(dst, c, dim, x);
+#pragma unroll
+        for (int u = 0; u < LOOKUP_AHEAD; ++u) {
+            if (x0 + u * LOOKUP_NT >= all) break;
+            const bool known = r[u] >= 0 && r[u] < n_rows;
+            float y[N];
+#pragma unroll
+            for (int e = 0; e < N; ++e) y[e] = known ? scale * v[u].get(e) : 0.0f;
+            store_values<To, N>(out + (first + i[u]) * ld_out, c[u], dim, y);
+        }
     }
 }
 
@@ -70,15 +93,29 @@ __device__ __forceinline__ int key_of(const int64_t* rows, const int* keys, int6
 }
 
 // Zeros for table rows, written by blocks behind those of a sort launch: the sort waits on latencies and leaves the
-// memory idle.  Rows [r0, r1) of `units` 16-bit units, `ld` units apart; a group of 1 << log_tpr threads takes a row.
+// memory idle.  Rows [r0, r1) of `units` 16-bit units, `ld` units apart: rows that lie back to back as one stretch from 16-byte
+// border to border (449640 x 597 fp16 row by row: 210 us, so 102), else a group of 1 << log_tpr threads takes a row.
 struct Fill {
     uint16_t* out;
     int64_t r0, r1, units, ld;
     int log_tpr;
 };
 __device__ static void fill_rows(const Fill& f, int64_t block, int64_t blocks, int nt) {
-    const int per = nt >> f.log_tpr;
     const u32x4 zero = {0u, 0u, 0u, 0u};
+    if (f.units == f.ld) {
+        uint16_t *lo = f.out + f.r0 * f.ld, *hi = f.out + f.r1 * f.ld;
+        uint16_t* border = (uint16_t*)(((uintptr_t)lo + 15) & ~(uintptr_t)15);
+        uint16_t* from = border < hi ? border : hi;
+        const int64_t pieces = (hi - from) / 8;
+        const int64_t share = (pieces + blocks - 1) / blocks, end = min((block + 1) * share, pieces);
+        for (int64_t i = block * share + threadIdx.x; i < end; i += nt) ((u32x4*)from)[i] = zero;
+        if (block == 0 && threadIdx.x < 8) {
+            if (lo + threadIdx.x < from) lo[threadIdx.x] = 0;
+            if (from + pieces * 8 + threadIdx.x < hi) from[pieces * 8 + threadIdx.x] = 0;
+        }
+        return;
+    }
+    const int per = nt >> f.log_tpr;
     for (int64_t r = f.r0 + block * per + (threadIdx.x >> f.log_tpr); r < f.r1; r += blocks * per) {
         uint16_t* dst = f.out + r * f.ld;
         for (int64_t c = (threadIdx.x & ((1 << f.log_tpr) - 1)) * 8; c < f.units; c += (int64_t)8 << f.log_tpr) {
@@ -496,7 +533,7 @@ __global__ void __launch_bounds__(JOIN_NT) seg_join_kernel(const int* __restrict
     }
 }
 
-// threads per row: a power of two that covers the row's pieces, at most a block
+// threads of a group that takes a row: a power of two that covers the row's pieces, at most a block
 static int log_threads(int pieces) {
     int l = 0;
     while (l < 8 && (1 << l) < pieces) ++l;
@@ -510,12 +547,17 @@ int launch_lookup(const void* table, int table_type, int64_t n_rows, int dim, in
         return with_type(out_type, [&](auto* to) -> int {
             typedef std::remove_pointer_t<decltype(ti)> Ti;
             typedef std::remove_pointer_t<decltype(to)> To;
-            const int l = log_threads((dim + Piece<Ti>::N - 1) / Piece<Ti>::N);
-            const int64_t most = ((int64_t)1 << 31) >> l;             // a launch holds fewer than 2^32 threads
+            // rows for one piece a thread, for four where that still leaves eight blocks a CU (88769 x 1672 fp32 by a block a
+            // row, two pieces a thread: 185 us, so 164)
+            const int64_t pieces = (dim + Piece<Ti>::N - 1) / Piece<Ti>::N;
+            const int each = n * pieces >= (int64_t)8 * ctx().num_cus * LOOKUP_AHEAD * LOOKUP_NT ? LOOKUP_AHEAD : 1;
+            const int take = ceil_div(each * LOOKUP_NT, pieces);
+            const uint32_t inverse = pieces > 1 ? (uint32_t)((((int64_t)1 << 32) + pieces - 1) / pieces) : 0;
+            const int64_t most = ((int64_t)1 << 23) * take;           // a launch holds fewer than 2^32 threads
             for (int64_t i = 0; i < n; i += most) {
                 const int64_t m = std::min(most, n - i);
-                hipLaunchKernelGGL((lookup_kernel<Ti, To>), dim3(ceil_div(m, 256 >> l)), dim3(256), 0, s, (const Ti*)table, n_rows, dim, ld, rows + i, m,
-                                   scale, (To*)out + i * ld_out, ld_out, l);
+                hipLaunchKernelGGL((lookup_kernel<Ti, To>), dim3(ceil_div(m, take)), dim3(LOOKUP_NT), 0, s, (const Ti*)table, n_rows, dim, ld, rows + i, m,
+                                   scale, (To*)out + i * ld_out, ld_out, take, (uint32_t)pieces, inverse);
                 VDB_HIP(hipGetLastError());
             }
             return VDB_OK;
@@ -567,11 +609,15 @@ static int launch_sort(const int64_t* rows, int64_t n, int64_t n_rows, const Gra
     *keys = w.keys[(p.passes + 1) & 1];
     *pos = w.pos[(p.passes + 1) & 1];
     if (n <= 0) return VDB_OK;
-    // blocks of 32 KB of zeros or more, at most eight a CU
+    // Zeros of 32 to 128 KB a block, two blocks a CU where there are that many, for rows that lie back to back (697 MB by 1024 threads:
+    // 133 us, with 32 or 256 KB a block 139 and 153, by two blocks a CU in turn 164); else blocks that go through the rows in turn.
     auto fill_blocks = [&](int64_t lo, int64_t hi, int threads) {
         fill.r0 = lo;
         fill.r1 = hi;
-        return (int)std::min<int64_t>(((hi - lo) * fill.units * 2 + 32767) / 32768, (int64_t)ctx().num_cus * 2048 / threads);
+        const int64_t bytes = (hi - lo) * fill.units * 2;
+        if (fill.units != fill.ld) return (int)std::min<int64_t>((bytes + 32767) / 32768, (int64_t)ctx().num_cus * 2048 / threads);
+        const int64_t share = std::min(std::max<int64_t>(bytes / (2 * ctx().num_cus), 1 << 15), (int64_t)1 << 17);
+        return (int)std::min<int64_t>((bytes + share - 1) / share, 1 << 20);
     };
     const int64_t fill_end = fill.out ? n_rows : 0;
     if (n <= COUNT_MAX) {
