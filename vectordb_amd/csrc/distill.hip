@@ -30,29 +30,6 @@ __device__ __forceinline__ MaxSum join(MaxSum a, MaxSum b, float c) {
     const float m = fmaxf(a.m, b.m), base = finite_base(m);
     return {m, a.s * exp2_fast((a.m - base) * c) + b.s * exp2_fast((b.m - base) * c)};
 }
-// Over a wave by data-parallel moves (rows of 16 lanes, then their last lanes passed on), for all lanes.
-template <int CTRL, int ROWS> __device__ __forceinline__ float moved(float v, float other) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(other), __float_as_int(v), CTRL, ROWS, 0xf, false));
-}
-__device__ __forceinline__ float last_lane(float v) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), 63)); }
-__device__ __forceinline__ float wave_sum(float v) {
-    v += moved<0x111, 0xf>(v, 0.0f);          // row_shr:1, 2, 4, 8
-    v += moved<0x112, 0xf>(v, 0.0f);
-    v += moved<0x114, 0xf>(v, 0.0f);
-    v += moved<0x118, 0xf>(v, 0.0f);
-    v += moved<0x142, 0xa>(v, 0.0f);          // row_bcast:15 into rows 1 and 3
-    v += moved<0x143, 0xc>(v, 0.0f);          // row_bcast:31 into rows 2 and 3
-    return last_lane(v);
-}
-__device__ __forceinline__ float wave_max(float v) {
-    v = fmaxf(v, moved<0x111, 0xf>(v, v));
-    v = fmaxf(v, moved<0x112, 0xf>(v, v));
-    v = fmaxf(v, moved<0x114, 0xf>(v, v));
-    v = fmaxf(v, moved<0x118, 0xf>(v, v));
-    v = fmaxf(v, moved<0x142, 0xa>(v, v));
-    v = fmaxf(v, moved<0x143, 0xc>(v, v));
-    return last_lane(v);
-}
 // A barrier for what was written to LDS; loads and stores of global memory stay under way.
 __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");

@@ -852,7 +852,7 @@ template <class T> __global__ void __launch_bounds__(ROW_NT) sample_kernel(const
 }
 
 // ---------------------------------------------------------------- long rows, by the whole chip
-// 1 sample_groups: the maxima of groups of 32 scores (and the histograms cleared)
+// 1 sample_groups: the maxima of groups of 32 scores and of the blocks' slices (and the histograms cleared)
 // 2 sample_pick (a block per row): rows that the best score or a list settles are finished from the maxima and the few
 //   groups that reach the bound; the others are marked
 // 3 sample_weigh: marked rows' weights, by parts of the row, and by distance from the best where top-p asks for it
@@ -870,9 +870,10 @@ struct RowState {
     uint32_t members;
 };
 static constexpr int PARTS = ROW_WAVES * GROUPS;                 // at most, per row
-static constexpr int PARTS_EACH = 4 * (STREAM_NT / 64);             // parts of a streaming block: four a wave
+static constexpr int WEIGH_PARTS = 4 * (FEW_NT / 64), ABOVE_PARTS = 4 * (STREAM_NT / 64);             // parts of a streaming block: four a wave
 struct SampleWork {
     float* group_max; int groups;    // [n][groups]
+    float* slice_max; int slices;    // [n][slices], slices as of fp32 rows at most
     RowState* state;                 // [n]
     u64* hist;                       // [n][BINS]
     u64* part; int parts, part_len;    // [n][PARTS], scores of a part (a multiple of 512)
@@ -891,6 +892,8 @@ static SampleWork sample_work(void* base, int64_t n, int64_t vocab) {
     w.part_len = (int)round_up64((vocab + PARTS - 1) / PARTS, 512);
     w.parts = (int)((vocab + w.part_len - 1) / w.part_len);
     w.group_max = (float*)take(n * w.groups * 4);
+    w.slices = ceil_div(vocab, STREAM_NT * Piece<float>::N * STREAM_PIECES);
+    w.slice_max = (float*)take(n * w.slices * 4);
     w.state = (RowState*)take(n * sizeof(RowState));
     w.hist = (u64*)take(n * BINS * 8);
     w.part = (u64*)take(n * PARTS * 8);
@@ -923,6 +926,7 @@ __global__ void __launch_bounds__(STREAM_NT) sample_groups_kernel(const T* __res
     }
     for (int b = slice * STREAM_NT + threadIdx.x; b < BINS; b += slices * STREAM_NT) w.hist[row * BINS + b] = 0;
     if (slice == 0 && threadIdx.x == 0) w.state[row] = RowState{};
+    float top = -INFINITY;
 #pragma unroll
     for (int j = 0; j < STREAM_PIECES; ++j) {
         const int at = first + j * STREAM_NT * N;
@@ -934,6 +938,16 @@ __global__ void __launch_bounds__(STREAM_NT) sample_groups_kernel(const T* __res
         m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x4E, 0xf, 0xf, false)));      // quad_perm:[2,3,0,1]
         if (N == 4) m = fmaxf(m, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(m), 0x141, 0xf, 0xf, false)));   // row_half_mirror
         if (threadIdx.x % (GROUP / N) == 0 && at < src.vocab) w.group_max[row * w.groups + at / GROUP] = m;
+        top = fmaxf(top, m);
+    }
+    __shared__ float tops[STREAM_NT / 64];
+    top = wave_max(top);
+    if ((threadIdx.x & 63) == 0) tops[threadIdx.x >> 6] = top;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+#pragma unroll
+        for (int i = 1; i < STREAM_NT / 64; ++i) top = fmaxf(top, tops[i]);
+        w.slice_max[row * w.slices + slice] = top;
     }
 }
 
@@ -1032,10 +1046,10 @@ template <class T> __device__ __forceinline__ void sample_pick(SampleShared& sh,
     }
 }
 
-// Parts [p0, p0 + PARTS_EACH) of a row, a run of them a wave: out[part] = the sum of f(piece, first element)
+// The parts of a row from p0 on, four a wave: out[part] = the sum of f(piece, first element)
 template <class T, class F, class P>
 __device__ __forceinline__ void stream_parts(const Source<T>& src, const SampleWork& work, int p0, u64* out, F&& f, P&& prologue) {
-    constexpr int N = Piece<T>::N, EACH = PARTS_EACH / (STREAM_NT / 64);
+    constexpr int N = Piece<T>::N, EACH = 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int first = p0 + EACH * wave, end = min(first + EACH, work.parts), steps = work.part_len / (64 * N);
     u64 sum = 0;
@@ -1048,27 +1062,29 @@ __device__ __forceinline__ void stream_parts(const Source<T>& src, const SampleW
                       sum = 0;
                   }, prologue);
 }
+// A row's weights by parts, and by distance from the best where top-p asks for it.
 template <class T>
-__global__ void __launch_bounds__(STREAM_NT) sample_weigh_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int cuts) {
+__device__ __forceinline__ void sample_weigh(SampleShared& sh, const T* __restrict__ scores, const SampleArgs& a, const SampleWork& work, int64_t row, int cut,
+                                             int slices) {
     constexpr int N = Piece<T>::N;
-    __shared__ double table[EXP_STEPS];
-    __shared__ u64 hist[BINS];
-    const int64_t row = blockIdx.x / cuts;
-    const int slice = (int)(blockIdx.x - row * cuts), mode = work.state[row].mode;
-    if (mode != ROW_SUM && mode != ROW_MASS) return;
-    const float best = work.state[row].best;
-    const Source<T> src(scores, a, row);
     const Settings set(a, row);
-    const FixedExp weigh(best, set.tau, a.shift, table);
+    const int mode = mode_of(set.tau, set.top_k, set.top_p, set.min_p);
+    if (mode != ROW_SUM && mode != ROW_MASS) return;
+    float best = -INFINITY;
+    for (int i = threadIdx.x & 63; i < slices; i += 64) best = fmaxf(best, work.slice_max[row * work.slices + i]);
+    best = wave_max(best);
+    if (!(fabsf(best) < INFINITY)) return;
+    const Source<T> src(scores, a, row);
+    const FixedExp weigh(best, set.tau, a.shift, sh.table);
     const u64 least_w = mode == ROW_SUM ? set.least_weight(a.shift) : 0;
-    stream_parts(src, work, slice * PARTS_EACH, work.part + row * PARTS, [&](const Piece<T>& v, int) {
+    stream_parts(src, work, cut * WEIGH_PARTS, work.part + row * PARTS, [&](const Piece<T>& v, int) {
         u64 w[N], sum = 0;
 #pragma unroll
         for (int e = 0; e < N; ++e) w[e] = weigh(v.get(e));
         if (mode == ROW_MASS) {
             // no branch between the scores: their chains of dependent steps overlap
 #pragma unroll
-            for (int e = 0; e < N; ++e) atomicAdd(&hist[weigh.bin(v.get(e))], w[e]);
+            for (int e = 0; e < N; ++e) atomicAdd(&sh.bin[weigh.bin(v.get(e))], w[e]);
         } else if (least_w) {
 #pragma unroll
             for (int e = 0; e < N; ++e) w[e] = w[e] >= least_w ? w[e] : 0;
@@ -1077,15 +1093,15 @@ __global__ void __launch_bounds__(STREAM_NT) sample_weigh_kernel(const T* __rest
         for (int e = 0; e < N; ++e) sum += w[e];
         return sum;
     }, [&] {
-        make_table<STREAM_NT>(table);
+        make_table<FEW_NT>(sh.table);
         if (mode == ROW_MASS)
-            for (int b = threadIdx.x; b < BINS; b += STREAM_NT) hist[b] = 0;
+            for (int b = threadIdx.x; b < BINS; b += FEW_NT) sh.bin[b] = 0;
         __syncthreads();
     });
     if (mode != ROW_MASS) return;
     __syncthreads();
-    for (int b = threadIdx.x; b < BINS; b += STREAM_NT)
-        if (hist[b]) atomicAdd(&work.hist[row * BINS + b], hist[b]);
+    for (int b = threadIdx.x; b < BINS; b += FEW_NT)
+        if (sh.bin[b]) atomicAdd(&work.hist[row * BINS + b], sh.bin[b]);
 }
 
 template <class T>
@@ -1108,7 +1124,7 @@ __global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __rest
     float lo, hi;
     weigh.bin_range(b, &lo, &hi);
     const float beyond = score_of(pattern(hi) + 1);              // the next larger score
-    stream_parts(src, work, slice * PARTS_EACH, work.part + row * PARTS, [&](const Piece<T>& v, int at) {
+    stream_parts(src, work, slice * ABOVE_PARTS, work.part + row * PARTS, [&](const Piece<T>& v, int at) {
         float top = v.get(0);
 #pragma unroll
         for (int e = 1; e < N; ++e) top = fmaxf(top, v.get(e));
@@ -1161,10 +1177,14 @@ __global__ void __launch_bounds__(STREAM_NT) sample_above_kernel(const T* __rest
     }
 }
 
+// Blocks below n: a row each.  The others, `cuts` a row: the weights of rows that ask for them.  A list takes one block as long
+// as the weights take the chip (25 and 15 us), so both go side by side.
 template <class T>
-__global__ void __launch_bounds__(FEW_NT) sample_pick_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work) {
+__global__ void __launch_bounds__(FEW_NT) sample_pick_kernel(const T* __restrict__ scores, SampleArgs a, SampleWork work, int n, int cuts, int slices) {
     __shared__ SampleShared sh;
-    sample_pick(sh, scores, a, work, blockIdx.x);
+    const int block = (int)blockIdx.x - n;
+    if (block < 0) return sample_pick(sh, scores, a, work, blockIdx.x);
+    sample_weigh(sh, scores, a, work, block / cuts, block % cuts, slices);
 }
 
 // The row's parts, of `total` after scan_parts: the one that holds the goal, read again by the first wave.
@@ -1298,12 +1318,10 @@ template <class T> static int launch_long_rows(const T* z, int64_t n, const Samp
     const RowMode mode = mode_of(a.temperature, a.top_k, a.top_p, a.min_p);
     const bool listed = all_known ? mode == ROW_LIST || mode == ROW_WHOLE
                                   : (!a.d_temperature && !(a.temperature > 0.0f)) || (!a.d_top_k && a.top_k >= 1) || (!a.d_top_p && a.top_p <= 0.0f);
-    hipLaunchKernelGGL(sample_pick_kernel<T>, rows, few, 0, s, z, a, w);
+    const int weigh_cuts = ceil_div(w.parts, WEIGH_PARTS), cuts = ceil_div(w.parts, ABOVE_PARTS);
+    hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)(listed ? n : n + n * weigh_cuts)), few, 0, s, z, a, w, (int)n, weigh_cuts, slices);
     VDB_HIP(hipGetLastError());
     if (!listed) {
-        const int cuts = ceil_div(w.parts, PARTS_EACH);
-        hipLaunchKernelGGL(sample_weigh_kernel<T>, dim3((unsigned)(n * cuts)), dim3(STREAM_NT), 0, s, z, a, w, cuts);
-        VDB_HIP(hipGetLastError());
         hipLaunchKernelGGL(sample_border_kernel<T>, rows, few, 0, s, z, a, w);
         VDB_HIP(hipGetLastError());
         if (a.d_top_p || a.top_p < 1.0f) {
