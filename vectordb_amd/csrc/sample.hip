@@ -853,12 +853,12 @@ template <class T> __global__ void __launch_bounds__(ROW_NT) sample_kernel(const
 
 // ---------------------------------------------------------------- long rows, by the whole chip
 // 1 sample_groups: the maxima of groups of 32 scores and of the blocks' slices (and the histograms cleared)
-// 2 sample_pick (a block per row): rows that the best score or a list settles are finished from the maxima and the few
-//   groups that reach the bound; the others are marked
-// 3 sample_weigh: marked rows' weights, by parts of the row, and by distance from the best where top-p asks for it
-// 4 sample_border (a block per row): the draw from the parts, or the bin in which the border of top-p lies
-// 5 sample_above: the weights above that bin by parts, and the bin's members
-// 6 sample_rest (a block per row): the border among the members and the draw; rows for which a list was too short go through
+// 2 sample_pick: a block per row finishes the rows that the best score or a list settles, from the maxima and the few groups
+//   that reach the bound, and marks the others; beside them, where settings ask for it, blocks of their own take the weights,
+//   by parts of the row, and by distance from the best where top-p asks for it
+// 3 sample_border (a block per row): the draw from the parts, or the bin in which the border of top-p lies
+// 4 sample_above: the weights above that bin by parts, and the bin's members
+// 5 sample_rest (a block per row): the border among the members and the draw; rows for which a list was too short go through
 //   all passes by one block
 static constexpr int GROUP = 32, STREAM_NT = 256, STREAM_PIECES = 4;
 enum RowMode { ROW_DONE = 0, ROW_WHOLE = 1, ROW_SUM = 2, ROW_MASS = 3, ROW_LIST = 4 };
