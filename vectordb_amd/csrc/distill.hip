@@ -6,9 +6,9 @@
 //   gradient   one pass that reads z and writes dz
 //   both       a row that fits a block's registers is read once: maximum, sum and gradient from there; longer rows take the
 //              two passes above
-// All are bound by HBM: n * vocab values read (twice for the two passes), and as many written for the gradient.  Rows need not be
-// aligned (a vocabulary of odd size): pieces are cut at 16-byte borders of memory, so the first and the last of a row
-// may be partial.
+// All are bound by HBM: n * vocab values read (twice for the two passes), and as many written for the gradient.  Measured: loss
+// of 4096 x 131072 bf16 184 us (5.8 TB/s), gradient of 5000 x 8191 bf16 34 us (5.0 TB/s), both of 4096 x 32768 bf16 110 us
+// (4.9 TB/s), of 8000 x 8000 bf16 50 us (5.3 TB/s).  Rows need not be aligned.
 #include "vdb_internal.h"
 #include "values.h"
 
@@ -454,17 +454,21 @@ template <class F> static int in_batches(int64_t n, F&& launch) {
     return VDB_OK;
 }
 
-// Parts of a row in pieces of 16 bytes: as many as fill the chip several times over, each of at least `least` pieces.
-static int parts_of(int64_t n, int64_t vocab, int per_piece, int64_t least, int64_t* part_pieces) {
+// Parts of a row in pieces of 16 bytes: as many as `blocks` allow, each of at least `least` pieces.
+static int parts_of(int64_t n, int64_t vocab, int per_piece, int64_t blocks, int64_t least, int64_t* part_pieces) {
     const int64_t pieces = vocab / per_piece + 2;                      // whatever the row's offset from a border
-    const int64_t want = std::max<int64_t>(1, (8 * (int64_t)ctx().num_cus + n - 1) / std::max<int64_t>(n, 1));
-    const int64_t parts = std::max<int64_t>(1, std::min({want, pieces / least, (int64_t)1024}));
+    const int64_t parts = std::max<int64_t>(1, std::min({blocks / std::max<int64_t>(n, 1), pieces / least, (int64_t)1024}));
     *part_pieces = (pieces + parts - 1) / parts;
     return (int)((pieces + *part_pieces - 1) / *part_pieces);
 }
-// The loss of few rows: by blocks of 1024 threads up to 2^17 scores each (one launch), in parts beyond that.
-static const int64_t LOSS_WIDE = 512, LOSS_PART = 16384;               // rows; pieces of a part
-static int loss_parts(int64_t n, int64_t vocab, int per_piece, int64_t* part_pieces) { return parts_of(n, vocab, per_piece, LOSS_PART, part_pieces); }
+// The loss: a block of 256 threads a row, of 1024 where there are few blocks (1 x 131072 bf16 9.9 us, 13.5 by 256), and parts of a
+// row, joined by a second launch, while they find a CU each (16 x 131072 fp32 7.9 us, 10.4 in one part; 500 x 32768 13.8,
+// 16.6 in two).
+static const int64_t LOSS_WIDE = 512, LOSS_PART = 4096;                // blocks; pieces of a part
+static int loss_parts(int64_t n, int64_t vocab, int per_piece, int64_t* part_pieces) {
+    const bool pays = vocab / per_piece + 2 >= 4 * LOSS_PART;          // two parts save less than the second launch takes
+    return parts_of(n, vocab, per_piece, pays ? ctx().num_cus : 0, LOSS_PART, part_pieces);
+}
 
 static int launch_loss(const void* scores, int type, int64_t n, int64_t vocab, int64_t ld, const Teacher& t, float tau, float* loss, float* stats,
                        void* work, hipStream_t s) {
@@ -491,7 +495,8 @@ static int launch_grad(const void* scores, int type, int64_t n, int64_t vocab, i
     return with_type(type, [&](auto* p) -> int {
         typedef std::remove_pointer_t<decltype(p)> T;
         int64_t part;
-        const int parts = parts_of(n, vocab, Piece<T>::N, AHEAD * GRAD_NT, &part);
+        // eight blocks a CU of a step of AHEAD pieces or more
+        const int parts = parts_of(n, vocab, Piece<T>::N, 8 * (int64_t)ctx().num_cus + n - 1, AHEAD * GRAD_NT, &part);
         return in_batches(n, [&](int64_t row0, unsigned rows) {
             hipLaunchKernelGGL(distill_grad_kernel<T>, dim3(rows, (unsigned)parts), dim3(GRAD_NT), t.lds(), s, (const T*)scores, row0, vocab, ld, t, tau, stats,
                                grad_loss, (T*)grad, ld_grad, part);
@@ -570,16 +575,17 @@ static int enter() {
 
 using namespace vdb;
 
-// the stats of a step in two passes, and the parts of long rows, which are no shorter
-static int64_t distill_stats_bytes(int64_t n) { return round_up64(n * 2 * (int64_t)sizeof(float), 256); }
+// the workspace: the stats of a step in two passes (whatever the type: fp32 rows have the most pieces), then the parts of long rows
+static int64_t distill_stats_bytes(int64_t n, int64_t vocab) {
+    return step_shape(n, vocab, 4).nt ? 0 : round_up64(n * 2 * (int64_t)sizeof(float), 256);
+}
 
 int vdb_distill_workspace(int64_t n, int64_t vocab, int64_t* bytes) {
     VDB_REQUIRE(bytes, "null pointer for the workspace size");
     VDB_REQUIRE(n >= 0 && vocab >= 1, "bad sizes for a distillation: %lld rows of %lld scores", (long long)n, (long long)vocab);
-    // whatever the type: rows of fp32 have the most pieces
     int64_t part;
     const int parts = loss_parts(n, vocab, 4, &part);
-    *bytes = (step_shape(n, vocab, 4).nt ? 0 : distill_stats_bytes(n)) + (parts > 1 ? n * parts * (int64_t)sizeof(MaxSum) : 0);
+    *bytes = distill_stats_bytes(n, vocab) + (parts > 1 ? n * parts * (int64_t)sizeof(MaxSum) : 0);
     return VDB_OK;
 }
 static int check_work(int64_t n, int64_t vocab, const void* d_work, int64_t work_bytes) {
@@ -600,7 +606,7 @@ int vdb_distill_dev(const void* d_scores, int type, int64_t n, int64_t vocab, in
     if (n == 0) return VDB_OK;
     VDB_TRY(enter());
     const Teacher t{d_teacher, d_rows, k, ld_teacher, ld_rows, d_teacher_lse, 1.0f / temperature};
-    return launch_loss(d_scores, type, n, vocab, ld, t, temperature, d_loss, d_stats, (char*)d_work + distill_stats_bytes(n), (hipStream_t)stream);
+    return launch_loss(d_scores, type, n, vocab, ld, t, temperature, d_loss, d_stats, (char*)d_work + distill_stats_bytes(n, vocab), (hipStream_t)stream);
 }
 
 int vdb_distill_grad_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int64_t ld, const float* d_teacher, const int64_t* d_rows, int k,
@@ -629,6 +635,6 @@ int vdb_distill_step_dev(const void* d_scores, int type, int64_t n, int64_t voca
     if (shape.nt)
         return launch_step(d_scores, type, n, vocab, ld, t, temperature, d_grad_loss, d_loss, d_stats, d_grad, ld_grad, shape, (hipStream_t)stream);
     float* stats = d_stats ? d_stats : (float*)d_work;
-    VDB_TRY(launch_loss(d_scores, type, n, vocab, ld, t, temperature, d_loss, stats, (char*)d_work + distill_stats_bytes(n), (hipStream_t)stream));
+    VDB_TRY(launch_loss(d_scores, type, n, vocab, ld, t, temperature, d_loss, stats, (char*)d_work + distill_stats_bytes(n, vocab), (hipStream_t)stream));
     return launch_grad(d_scores, type, n, vocab, ld, t, temperature, stats, d_grad_loss, d_grad, ld_grad, (hipStream_t)stream);
 }
