@@ -669,6 +669,45 @@ def test_refusals(ops):
             call()
 
 
+# ---------------------------------------------------------------- workspaces
+def test_workspaces_are_kept_to(ops, monkeypatch):
+    """No call writes before or behind the bytes that its workspace function names, and none reads what was there before."""
+    guards = []
+
+    def workspace(fn, *sizes):
+        need = ops._workspace_bytes(fn, *sizes)
+        t = torch.randint(0, 256, (need + 1024,), device="cuda", dtype=torch.uint8)
+        guards.append((t, t.clone(), need, fn, sizes))
+        return t, t.data_ptr() + 512, need
+
+    def run(call):
+        guards.clear()
+        monkeypatch.setattr(ops, "_workspace", workspace)
+        got = call()
+        monkeypatch.undo()
+        want = call()
+        for t, before, need, fn, sizes in guards:
+            assert torch.equal(t[:512], before[:512]) and torch.equal(t[512 + need:], before[512 + need:]), (fn, sizes)
+        for x, y in zip(got, want):
+            assert torch.equal(x, y), guards[0][3:]
+
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    r = lambda *s: torch.randn(*s, device="cuda", generator=g)               # noqa: E731
+    for n, n_rows, dim in ((1, 5, 3), (33, 7, 9), (100, 1000, 5), (4097, 90, 33), (12288, 60, 16), (12289, 60, 16), (20000, 300000, 6), (70000, 5000, 130)):
+        x, at = r(n, dim), torch.randint(-1, n_rows, (n,), device="cuda", generator=g)
+        run(lambda: (ops.lookup_grad(x, at, n_rows),))
+    for dtype in (torch.float32, torch.bfloat16):
+        for n, vocab in ((1, 10), (5, 32768), (3, 65527), (3, 65528), (2, 65537), (1, 131072), (130, 70001), (600, 65536), (600, 65540), (1, 1000003)):
+            z, t, at, w = r(n, vocab).to(dtype), r(n, 4), torch.randint(-1, vocab, (n, 4), device="cuda", generator=g), r(n)
+            run(lambda: ops.distill(z, t, at))
+            run(lambda: ops.distill_step(z, t, at, w))
+        for n, vocab in ((3, 32768), (3, 32769), (2, 40_000), (17, 131072), (2, 600_001)):
+            z, u = r(n, vocab).to(dtype) * 2, torch.rand(n, device="cuda", generator=g)
+            for kw in ({}, {"top_k": 90}, {"top_p": 0.9}, {"min_p": 0.001}):
+                run(lambda: ops.sample(z, u, **kw))
+
+
 # ---------------------------------------------------------------- together
 def together(ops, table, tokens, queries, teacher, at, weight, uniforms):
     """A training step of the rows and an answer: look rows up, score them, distill, send the gradient back to the rows; draw from the scores."""
