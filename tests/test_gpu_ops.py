@@ -220,6 +220,39 @@ def test_lookup_dimensions(ops, dim, tin, tout):
         assert torch.equal(room[:, :dim], want) and bool((room[:, dim:] == 7).all()), n
 
 
+@pytest.mark.parametrize("n", [1, 2, 63, 64, 65, 127, 128, 129])
+@pytest.mark.parametrize("kind,tout", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16")])
+def test_lookup_grad_few(ops, n, kind, tout):
+    """Few positions: rows of their own, one row for all, two that take turns, none; tables of one row to many."""
+    rng = rng_for("few", n, kind)
+    for n_rows, dim in ((1, 5), (70, 3), (500, 200), (300, 1030), (20, 4099), (3000, 390)):
+        x = rng.randint(-3, 4, (n, dim)).astype(np.float32)
+        grad = padded(cuda(x, TYPES[kind]), 3, 1)
+        for rows in (rng.permutation(np.arange(n) % n_rows), np.full(n, n_rows - 1), np.arange(n) % 2, rng.randint(-2, n_rows + 2, n), np.full(n, -1)):
+            want = np.zeros((n_rows, dim))
+            known = (rows >= 0) & (rows < n_rows)
+            np.add.at(want, rows[known], x[known])
+            at = cuda(rows.astype(np.int64))
+            room = torch.full((n_rows, dim + 1), 7.0, device="cuda", dtype=TYPES[tout])
+            ops.lookup_grad(grad, at, n_rows, out=room[:, :dim])
+            assert (f64(room[:, :dim]) == want).all() and bool((room[:, dim:] == 7).all()), (n_rows, dim)
+            ops.lookup_grad(grad, at, n_rows, out=room[:, :dim], accumulate=True)
+            assert (f64(room[:, :dim]) == 2 * want).all() and bool((room[:, dim:] == 7).all()), (n_rows, dim)
+
+
+def test_lookup_grad_few_into_many(ops):
+    """Few positions and a table whose zeros take longer than they do."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(4)
+    for n, n_rows, dim in ((1, 90_000, 200), (20, 90_000, 200), (128, 17_000, 1000)):
+        x = torch.randint(-3, 4, (n, dim), device="cuda", generator=g).float()
+        at = torch.randint(-1, 9, (n,), device="cuda", generator=g) * (n_rows // 9)
+        want = torch.zeros(n_rows, dim, device="cuda")
+        want.index_add_(0, at[at >= 0], x[at >= 0])
+        assert torch.equal(ops.lookup_grad(x, at, n_rows), want)
+        assert torch.equal(ops.lookup_grad(x, at, n_rows, out=want.clone(), accumulate=True), 2 * want)
+
+
 def test_lookup_grad_differences(ops):
     """The gradient of sum(w * lookup(table)) against the quotient of differences: linear, so the quotient is exact but for rounding."""
     rng = rng_for("differences")

@@ -38,8 +38,8 @@ SAMPLE = dict(scores=P, t=0, n=4, vocab=50, ld=50, sf=0, u=P, dt=None, tau=1.0, 
     ("vdb_lookup_grad_dev", GRAD, dict(gt=9), "value type"), ("vdb_lookup_grad_dev", GRAD, dict(dim=0), "bad sizes"),
     ("vdb_lookup_grad_dev", GRAD, dict(n=1 << 31), "bad sizes"), ("vdb_lookup_grad_dev", GRAD, dict(ldo=4), "leading dimensions"),
     ("vdb_lookup_grad_dev", GRAD, dict(ld=-1), "leading dimensions"), ("vdb_lookup_grad_dev", GRAD, dict(grad=None), "null pointer"),
-    ("vdb_lookup_grad_dev", GRAD, dict(out=None), "null pointer"), ("vdb_lookup_grad_dev", GRAD, dict(size=16), "workspace"),
-    ("vdb_lookup_grad_dev", GRAD, dict(work=None), "workspace"),
+    ("vdb_lookup_grad_dev", GRAD, dict(out=None), "null pointer"), ("vdb_lookup_grad_dev", GRAD, dict(n=500, size=16), "workspace"),
+    ("vdb_lookup_grad_dev", GRAD, dict(n=500, work=None), "workspace"),
     ("vdb_distill_dev", DISTILL, dict(t=3), "value type"), ("vdb_distill_dev", DISTILL, dict(vocab=0), "bad sizes"),
     ("vdb_distill_dev", DISTILL, dict(k=_native.DISTILL_MAX_K + 1), "slots"), ("vdb_distill_dev", DISTILL, dict(ldr=-3), "slots"),
     ("vdb_distill_dev", DISTILL, dict(tau=0.0), "temperature"), ("vdb_distill_dev", DISTILL, dict(tau=float("nan")), "temperature"),
