@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(COUNT_NT) sort_count_kernel(const int64_t* __r
 }
 
 // ---------------------------------------------------------------- sums of the sorted rows
-// Positions of a chunk: the rows of a batch of SEG_BATCH are in flight together.  Chunks of 32 where that fills the chip,
-// else of 8 (10240 rows of 384 values: 22 us with 32).
+// The rows of a batch of SEG_BATCH positions are in flight together; a chunk is as many batches as still fill the chip, one at
+// least (10240 rows of 384 values: 22 us with four).
 static constexpr int SEG_BATCH = 8;
 
 // first position whose key is not below r, found by a whole wave: 64 probes a step (n and keys are below 2^31)
