@@ -381,6 +381,34 @@ def test_distill_long_rows(ops, n, vocab, kind):
     assert torch.equal(room.float(), outside.float())                           # in place, and nothing beside the rows
 
 
+@pytest.mark.parametrize("vocab", [1, 40, 900, 5000, 40_000])
+def test_distill_long_lists(ops, vocab):
+    """Lists of 1024 slots, longer than some rows: every place named many times, or one place by all."""
+    rng = rng_for("long lists", vocab)
+    n, k = 5, 1024
+    z, t, at = distill_inputs(rng, n, vocab, k, torch.float32, ragged=False)
+    at[1] = vocab - 1
+    at[2, 100:] = -1
+    at[3, ::2] = at[3, 1::2]
+    w = rng.randn(n).astype(np.float32)
+    loss, stats = ops.distill(z, cuda(t), cuda(at))
+    grad = ops.distill_grad(z, cuda(t), cuda(at), stats, cuda(w))
+    loss2, grad2 = ops.distill_step(z, cuda(t), cuda(at), cuda(w))
+    for i in range(n):
+        r = R.distill_row(f64(z[i]), t[i], at[i], 1.0)
+        e_logs, e_lp, filled = distill_bounds(r, t[i].astype(np.float64), 1.0, vocab, k)
+        # as in test_distill; up to k probabilities are added up one by one in a place
+        worst = float(e_lp.max())
+        for got in (loss, loss2):
+            gap = np.abs(r["logp"][filled] - (r["d"][at[i][filled]] - r["logs"]))
+            tol = float((r["p"][filled] * (worst + e_logs + U * 200 + gap * (worst + 40 * U))).sum()) + 4 * U * abs(r["loss"])
+            assert abs(float(got[i]) - r["loss"]) <= tol, (i, float(got[i]), r["loss"], tol)
+        d = np.where(np.isfinite(r["d"]), -r["d"], 0.0)
+        tol = np.abs(w[i]) * (r["mass"] * r["q"] * (5 * U * d + e_logs + worst + (k / 64 + 24) * U) + r["target"] * (worst + (k + 8) * U))
+        for got in (grad, grad2):
+            check(f64(got[i]), w[i] * r["grad"], tol + half_step(torch.float32, np.abs(w[i] * r["grad"]) + tol), i)
+
+
 def test_distill_many_rows(ops):
     """More rows than one launch takes: the last ones are what they are by themselves."""
     n, vocab, k = (1 << 21) + 7, 9, 3
@@ -811,6 +839,38 @@ def test_captured_and_replayed(ops):
             torch.cuda.synchronize()
             for a, b in zip(outs, want):
                 assert torch.equal(a, b), (turn, k)
+
+
+def test_captured_large(ops):
+    """Calls of several launches, captured together and replayed with new inputs and eager work between, against eager results."""
+    def inputs(seed):
+        g = torch.Generator(device="cuda")
+        g.manual_seed(seed)
+        r = lambda *s: torch.randn(*s, device="cuda", generator=g)           # noqa: E731
+        return (r(20000, 24), torch.randint(-1, 9000, (20000,), device="cuda", generator=g), r(3, 140_001) * 2, r(3, 6),
+                torch.randint(-1, 140_001, (3, 6), device="cuda", generator=g), torch.rand(3, device="cuda", generator=g))
+
+    def calls(x, at, z, t, rows, u):
+        return (ops.lookup_grad(x, at, 9000), ops.lookup_grad(x[:3000], at[:3000], 9000), *ops.distill(z, t, rows), *ops.distill_step(z, t, rows, u),
+                *ops.sample(z, u, top_p=0.9), *ops.sample(z[:, :20_000], u, top_p=0.8), *ops.sample(z, u, top_k=300))
+
+    ins = [t.clone() for t in inputs(1)]
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        calls(*ins)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        outs = calls(*ins)
+    for turn in range(4):
+        for t, new in zip(ins, inputs(50 + turn)):
+            t.copy_(new)
+        g.replay()
+        want = calls(*ins)
+        torch.cuda.synchronize()
+        for k, (a, b) in enumerate(zip(outs, want)):
+            assert torch.equal(a, b), (turn, k)
 
 
 def test_two_streams(ops):

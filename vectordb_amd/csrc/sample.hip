@@ -1303,9 +1303,16 @@ template <class T> __global__ void __launch_bounds__(ROW_NT) sample_rest_kernel(
 }
 
 // Short rows go to one block each: what the other form saves in passes it loses in launches.  Rows of 32768 scores, by one
-// block each and by the whole chip: one row with top-k 50 12 and 13 us, top-p 0.9 44 and 30 us; 256 rows with settings of
-// every kind 49 and 60 us, 1024 rows 106 and 100 us.
+// block each and by the whole chip: one row with top-k 50 11 and 13 us, 256 rows with settings of every kind 46 and 57 us, 1024
+// rows 106 and 100 us.  Few rows with top-p alone take two passes of weights, for which one block is slow: 1, 16, 64, 128 rows
+// of 32768 44, 45, 45, 46 us by a block and 31, 33, 36, 42 by the chip, of 20000 37, 37, 37, 38 and 31, 33, 35, 40, of 12000
+// 26 to 28 and 31 to 36.
 static bool by_whole_chip(int64_t vocab) { return vocab > 32768; }
+static bool few_rows(int64_t n, int64_t vocab) { return n <= 64 && vocab > 16384; }
+static bool whole_chip_pays(int64_t n, const SampleArgs& a) {
+    const bool top_p_alone = !a.d_top_k && a.top_k <= 0 && (a.d_top_p || (a.top_p > 0.0f && a.top_p < 1.0f)) && (a.d_temperature || a.temperature > 0.0f);
+    return by_whole_chip(a.vocab) || (few_rows(n, a.vocab) && top_p_alone);
+}
 static const int64_t SAMPLE_BATCH = 1024;           // rows at a time by the whole chip: bounds the workspace (59 MB at 131072 scores)
 
 template <class T> static int launch_long_rows(const T* z, int64_t n, const SampleArgs& a, const SampleWork& w, hipStream_t s) {
@@ -1335,7 +1342,7 @@ template <class T> static int launch_long_rows(const T* z, int64_t n, const Samp
 }
 
 template <class T> static int launch_sample(const T* z, int64_t n, const SampleArgs& a, void* d_work, hipStream_t s) {
-    const bool whole_chip = by_whole_chip(a.vocab);
+    const bool whole_chip = whole_chip_pays(n, a);
     const int64_t batch = whole_chip ? SAMPLE_BATCH : (int64_t)1 << 21;           // a launch holds fewer than 2^32 threads
     const SampleWork w = whole_chip ? sample_work(d_work, std::min(n, batch), a.vocab) : SampleWork{};
     for (int64_t r = 0; r < n; r += batch) {
@@ -1366,7 +1373,7 @@ int vdb_sample_workspace(int64_t n, int64_t vocab, int64_t* bytes) {
     VDB_REQUIRE(bytes, "null pointer for the workspace size");
     VDB_REQUIRE(n >= 0 && vocab >= 1 && vocab <= ((int64_t)1 << 24), "bad sizes for sampling: %lld rows of %lld scores (at most 2^24)", (long long)n,
                 (long long)vocab);
-    *bytes = by_whole_chip(vocab) ? sample_work(nullptr, std::min(n, SAMPLE_BATCH), vocab).bytes : 0;
+    *bytes = by_whole_chip(vocab) || few_rows(n, vocab) ? sample_work(nullptr, std::min(n, SAMPLE_BATCH), vocab).bytes : 0;
     return VDB_OK;
 }
 
