@@ -482,7 +482,7 @@ int vdb_distill_step_dev(const void* d_scores, int type, int64_t n, int64_t voca
  * NULL) is the log of the drawn row's share of the remaining weights.  Settings come per row (device arrays, where
  * given) or as one value for all.  mask: packed words as everywhere (bit v % 32 of word v / 32 set = may be drawn),
  * rows `mask_ld` words apart, 0 = one mask for all; NULL = no mask.  smaller_first != 0: the scores are distances
- * (z = -score).  vocab <= 2^24. */
+ * (z = -score).  vocab <= 2^24.  With a top_k, rows of up to 32768 scores need no workspace whatever the size named. */
 int vdb_sample_workspace(int64_t n, int64_t vocab, int64_t* bytes);
 int vdb_sample_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int64_t ld, int smaller_first, const float* d_uniform,
                    const float* d_temperature, float temperature, const int32_t* d_top_k, int top_k, const float* d_top_p, float top_p,

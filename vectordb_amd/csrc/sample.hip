@@ -1388,16 +1388,17 @@ int vdb_sample_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int
     VDB_REQUIRE(mask_ld == 0 || mask_ld >= (vocab + 31) / 32, "a mask over %lld scores takes %lld words a row, its rows lie %lld apart", (long long)vocab,
                 (long long)((vocab + 31) / 32), (long long)mask_ld);
     VDB_REQUIRE(n == 0 || (d_scores && d_uniform && d_out_row), "null pointer in sampling from %lld rows", (long long)n);
+    int bits = 0;
+    while (((int64_t)1 << bits) < vocab) ++bits;
+    const SampleArgs a{vocab, ld, smaller_first, d_uniform, d_temperature, temperature, d_top_k, top_k, d_top_p, top_p, d_min_p, min_p,
+                       d_mask, mask_ld, d_out_row, d_out_logp, std::min(52, 62 - bits)};
+    if (!whole_chip_pays(n, a)) need = 0;
     VDB_REQUIRE(work_bytes >= need && (d_work || need == 0), "the workspace of %lld bytes is too small for this sampling (%lld needed)",
                 (long long)work_bytes, (long long)need);
     VDB_REQUIRE(aligned_work(d_work), "a workspace begins at a multiple of 16 bytes");
     if (n == 0) return VDB_OK;
     VDB_TRY(ensure_init());
     (void)hipSetDevice(ctx().device);
-    int bits = 0;
-    while (((int64_t)1 << bits) < vocab) ++bits;
-    const SampleArgs a{vocab, ld, smaller_first, d_uniform, d_temperature, temperature, d_top_k, top_k, d_top_p, top_p, d_min_p, min_p,
-                       d_mask, mask_ld, d_out_row, d_out_logp, std::min(52, 62 - bits)};
     return with_type(type, [&](auto* p) -> int {
         typedef std::remove_pointer_t<decltype(p)> T;
         return launch_sample((const T*)d_scores, n, a, d_work, (hipStream_t)stream);

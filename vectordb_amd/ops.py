@@ -302,7 +302,8 @@ def sample(scores: torch.Tensor, uniforms: torch.Tensor, temperature: Union[floa
         mask_ld = mask_words.stride(0) if mask_words.dim() == 2 and n > 1 else 0
     out = torch.empty(n, device=_where, dtype=torch.int64)
     logp = torch.empty(n, device=_where, dtype=torch.float32)
-    keep, work, size = _workspace("vdb_sample_workspace", n, vocab)
+    # short rows with a top-k need none
+    keep, work, size = (None, None, 0) if vocab <= 32768 and (k is not None or kv > 0) else _workspace("vdb_sample_workspace", n, vocab)
     _native.check(_lib.vdb_sample_dev(_p(scores), code, n, vocab, ld, int(distances), _p(uniforms), t, tv, k, kv, p, pv, m, mv,
                                                 _p(mask_words), mask_ld, _p(out), _p(logp), work, size, _stream()))
     return out, logp
