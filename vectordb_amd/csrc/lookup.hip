@@ -339,7 +339,7 @@ template <class To, int N> __device__ __forceinline__ void put_row(To* row, int 
 // sums of a part of a row lie in whole pieces
 __host__ __device__ static inline int64_t part_pitch(int dim) { return ((int64_t)dim + 7) & ~7; }
 
-static constexpr int ZERO_ROWS = 64;
+static constexpr int ZERO_ROWS = 64;                        // table rows that a block writes zeros to, at most
 
 // zeros to those of the `count` table rows from r0 on that are not named
 template <class To>
@@ -381,26 +381,26 @@ template <class T> __device__ __forceinline__ void drop_neighbours(int skip, Pie
 // Blocks below zero_from: a group of 1 << log_tpr threads takes the chunk g of sorted positions; columns in slices of
 // blockIdx.y.  A row that neither starts before the chunk nor goes on behind it is finished here; the part of a row that
 // started before goes to part[g][0], of one that starts here and goes on to part[g][1].
-// The other blocks write zeros to those of ZERO_ROWS table rows that no position names (slice 0 alone).
+// The other blocks write zeros to those of zero_each table rows that no position names (slice 0 alone).
 template <class Tg, class To>
 __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ grad, int64_t ld, const int* __restrict__ keys,
                                                       const int* __restrict__ pos, int64_t n, float scale, To* __restrict__ out,
                                                       int64_t n_rows, int dim, int64_t ld_out, int accumulate, float* __restrict__ part,
-                                                      int chunk, int64_t chunks, int log_tpr, int zero_from, int log_zero) {
+                                                      int chunk, int64_t chunks, int log_tpr, int zero_from, int log_zero, int zero_each) {
     if ((int)blockIdx.x >= zero_from) {
         if (blockIdx.y) return;
         __shared__ int64_t range[2];
         __shared__ int named[ZERO_ROWS];
-        const int64_t r0 = (int64_t)((int)blockIdx.x - zero_from) * ZERO_ROWS;
+        const int64_t r0 = (int64_t)((int)blockIdx.x - zero_from) * zero_each;
         if (threadIdx.x < ZERO_ROWS) named[threadIdx.x] = 0;
         if (threadIdx.x < 128) {
-            const int64_t at = lower_bound_wave(keys, n, r0 + (threadIdx.x >> 6) * ZERO_ROWS);
+            const int64_t at = lower_bound_wave(keys, n, r0 + (threadIdx.x >> 6) * zero_each);
             if ((threadIdx.x & 63) == 0) range[threadIdx.x >> 6] = at;
         }
         __syncthreads();
         if (range[1] - range[0] <= 8 * 256) {
             for (int64_t p = range[0] + threadIdx.x; p < range[1]; p += 256) named[keys[p] - r0] = 1;
-        } else if (threadIdx.x < ZERO_ROWS) {            // rows named many times: each looks for itself (131072 positions of 10 rows: 161 us to go through)
+        } else if ((int)threadIdx.x < zero_each) {            // rows named many times: each looks for itself (131072 positions of 10 rows: 161 us to go through)
             const int64_t r = r0 + threadIdx.x;
             uint32_t a = (uint32_t)range[0], b = (uint32_t)range[1];
             while (a < b) {
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ gra
             named[threadIdx.x] = a < (uint32_t)range[1] && keys[a] == r;
         }
         __syncthreads();
-        zero_rows(named, out, r0, ZERO_ROWS, n_rows, dim, ld_out, log_zero, 256);
+        zero_rows(named, out, r0, zero_each, n_rows, dim, ld_out, log_zero, 256);
         return;
     }
     constexpr int N = Piece<Tg>::N;
@@ -647,9 +647,10 @@ struct GradWork {
 static int seg_chunk(int64_t n, int dim) {
     if (n <= 32) return 32;                                           // a single chunk needs no second launch
     const int64_t lanes = n * ((dim + 3) / 4);
-    // 131072 x 2048: parts written and joined cost 37 us with chunks of 32, 20 us with 64, the sums 348 and 352 us
+    // 131072 x 2048: parts written and joined cost 37 us with chunks of 32, 20 us with 64, the sums 348 and 352 us; 131072 x 64 as
+    // a whole 59 us with 256 K lanes or more, 54 with 128 K, 56 with 64 K
     for (int chunk = 64; chunk > 8; chunk >>= 1)
-        if (lanes / chunk >= (int64_t)256 * 1024) return chunk;
+        if (lanes / chunk >= (int64_t)128 * 1024) return chunk;
     return 8;
 }
 // Whether the whole table is zeroed beside the sort, and the named rows written over it: where those are few (10240 x 384
@@ -762,9 +763,11 @@ static int launch_lookup_grad(const void* grad, int grad_type, int64_t ld, const
             typedef std::remove_pointer_t<decltype(tg)> Tg;
             const int pieces = (dim + Piece<Tg>::N - 1) / Piece<Tg>::N, l = log_threads(pieces);
             const int lz = log_threads((dim + Piece<To>::N - 1) / Piece<To>::N);
-            const int sums = ceil_div(chunks, 256 >> l), zeros = accumulate || filled ? 0 : ceil_div(n_rows, ZERO_ROWS);
+            // two blocks a CU for the zeros of small tables (1963 x 469 bf16 into 4316 rows: 22 us with 64 rows each, so 18)
+            const int zero_each = (int)std::min<int64_t>(std::max<int64_t>(n_rows / (2 * ctx().num_cus), 8), ZERO_ROWS);
+            const int sums = ceil_div(chunks, 256 >> l), zeros = accumulate || filled ? 0 : ceil_div(n_rows, zero_each);
             hipLaunchKernelGGL((seg_sum_kernel<Tg, To>), dim3(sums + zeros, ceil_div(pieces, 1 << l)), dim3(256), 0, s, (const Tg*)grad, ld, keys, pos,
-                               n, scale, (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks, l, sums, lz);
+                               n, scale, (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks, l, sums, lz, zero_each);
             VDB_HIP(hipGetLastError());
             if (chunks > 1) {
                 hipLaunchKernelGGL((seg_join_kernel<To>), dim3(ceil_div(chunks - 1, JOIN_CHUNKS), ceil_div(dim, 256)), dim3(JOIN_NT), 0, s, keys, n, scale,
