@@ -66,7 +66,7 @@ __global__ void __launch_bounds__(LOOKUP_NT) lookup_kernel(const Ti* __restrict_
 }
 
 // ---------------------------------------------------------------- stable radix sort of the positions by row number
-static constexpr int SORT_NT = 256, SORT_WAVES = SORT_NT / 64, SORT_MAX_BITS = 10;
+static constexpr int SORT_NT = 256, SORT_WAVES = SORT_NT / 64, SORT_MAX_BITS = 10, SORT_BLOCKS = 512;
 
 struct SortPlan {
     int passes, bits;          // digits of `bits` bits; keys are 0 .. n_rows (n_rows = no row)
@@ -80,8 +80,8 @@ static SortPlan sort_plan(int64_t n, int64_t n_rows) {
     p.passes = (key_bits + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     p.bits = (key_bits + p.passes - 1) / p.passes;
     // a wave takes its keys 64 at a time, each step waiting for the last: few of them, until the blocks' histograms
-    // would outgrow what they save (512 blocks)
-    p.wave_keys = std::max<int64_t>(128, round_up64((n + 512 * SORT_WAVES - 1) / (512 * SORT_WAVES), 64));
+    // would outgrow what they save
+    p.wave_keys = std::max<int64_t>(128, round_up64((n + SORT_BLOCKS * SORT_WAVES - 1) / (SORT_BLOCKS * SORT_WAVES), 64));
     p.blocks = (int)((n + p.wave_keys * SORT_WAVES - 1) / (p.wave_keys * SORT_WAVES));
     return p;
 }
@@ -141,20 +141,27 @@ __global__ void __launch_bounds__(SORT_NT) sort_hist_kernel(const int64_t* __res
     for (int d = threadIdx.x; d < bins; d += SORT_NT) hist[(int64_t)d * blocks + blockIdx.x] = cnt[d];
 }
 
-// one wave per digit: exclusive prefix of its counts over the blocks, and their total
+// inclusive prefix over a wave
+__device__ __forceinline__ int wave_prefix(int v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int t = __shfl_up(v, o);
+        if (lane >= o) v += t;
+    }
+    return v;
+}
+// one wave per digit: exclusive prefix of its counts over the blocks, all loaded at once, and their total
 __global__ void __launch_bounds__(64) sort_scan_kernel(int* __restrict__ hist, int blocks, int* __restrict__ totals) {
     int* h = hist + (int64_t)blockIdx.x * blocks;
-    int run = 0;
-    for (int b0 = 0; b0 < blocks; b0 += 64) {
-        const int b = b0 + threadIdx.x;
-        const int v = b < blocks ? h[b] : 0;
-        int s = v;
+    int v[SORT_BLOCKS / 64], run = 0;
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int t = __shfl_up(s, o);
-            if ((int)threadIdx.x >= o) s += t;
-        }
-        if (b < blocks) h[b] = run + s - v;
+    for (int j = 0; j < SORT_BLOCKS / 64; ++j) v[j] = j * 64 + (int)threadIdx.x < blocks ? h[j * 64 + threadIdx.x] : 0;
+#pragma unroll
+    for (int j = 0; j < SORT_BLOCKS / 64; ++j) {
+        if (j * 64 >= blocks) break;
+        const int s = wave_prefix(v[j]);
+        if (j * 64 + (int)threadIdx.x < blocks) h[j * 64 + threadIdx.x] = run + s - v[j];
         run += __shfl(s, 63);
     }
     if (threadIdx.x == 0) totals[blockIdx.x] = run;
@@ -184,36 +191,40 @@ __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __
                                                                int* __restrict__ keys_out, int* __restrict__ pos_out, int blocks, Fill fill) {
     extern __shared__ int lds[];
     if ((int)blockIdx.x >= blocks) return fill_rows(fill, (int)blockIdx.x - blocks, (int)gridDim.x - blocks, SORT_NT);
+    constexpr int MOST = (1 << SORT_MAX_BITS) / SORT_NT;
     const int bins = 1 << bits;
     int* start = lds;                         // [SORT_WAVES][bins]
-    int* scan = lds + SORT_WAVES * bins;      // [SORT_NT]
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // a contiguous run of digits per thread: their totals and what the blocks before have of them
+    const int per = (bins + SORT_NT - 1) / SORT_NT;
+    int total[MOST], before[MOST];
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) {
+        const int d = tid * per + j;
+        const bool mine = j < per && d < bins;
+        total[j] = mine ? totals[d] : 0;
+        before[j] = mine ? hist[(int64_t)d * blocks + blockIdx.x] : 0;
+    }
     for (int d = tid; d < SORT_WAVES * bins; d += SORT_NT) start[d] = 0;
     __syncthreads();
     const int64_t lo = ((int64_t)blockIdx.x * SORT_WAVES + wave) * wave_keys, hi = min(lo + wave_keys, n);
     int* mine = start + wave * bins;
     for (int64_t i = lo + lane; i < hi; i += 64) atomicAdd(&mine[(key_of(rows, keys, i, n_rows) >> shift) & (bins - 1)], 1);
-    // exclusive prefix of the digit totals: a contiguous run of digits per thread, then over the threads
-    const int per = (bins + SORT_NT - 1) / SORT_NT;
+    __shared__ int wave_total[SORT_WAVES];
     int sum = 0;
-    for (int j = 0; j < per; ++j) {
-        const int d = tid * per + j;
-        if (d < bins) sum += totals[d];
-    }
-    scan[tid] = sum;
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) sum += total[j];
+    const int upto = wave_prefix(sum);
+    if (lane == 63) wave_total[wave] = upto;
     __syncthreads();
-    for (int o = 1; o < SORT_NT; o <<= 1) {
-        const int t = tid >= o ? scan[tid - o] : 0;
-        __syncthreads();
-        scan[tid] += t;
-        __syncthreads();
-    }
-    int run = tid > 0 ? scan[tid - 1] : 0;
-    for (int j = 0; j < per; ++j) {
+    int run = upto - sum;
+    for (int w = 0; w < wave; ++w) run += wave_total[w];
+#pragma unroll
+    for (int j = 0; j < MOST; ++j) {
         const int d = tid * per + j;
-        if (d >= bins) break;
-        int at = run + hist[(int64_t)d * blocks + blockIdx.x];
-        run += totals[d];
+        if (j >= per || d >= bins) break;
+        int at = run + before[j];
+        run += total[j];
         for (int w = 0; w < SORT_WAVES; ++w) {
             const int c = start[w * bins + d];
             start[w * bins + d] = at;
@@ -717,7 +728,7 @@ static int launch_sort(const int64_t* rows, int64_t n, int64_t n_rows, const Gra
         hipLaunchKernelGGL(sort_scan_kernel, dim3(bins), dim3(64), 0, s, w.hist, p.blocks, w.totals);
         VDB_HIP(hipGetLastError());
         extra = fill_blocks(fill_end * (2 * pass + 1) / shares, fill_end * (2 * pass + 2) / shares, SORT_NT);
-        hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks + extra), dim3(SORT_NT), (SORT_WAVES * bins + SORT_NT) * 4, s, src_rows, src_keys, src_pos,
+        hipLaunchKernelGGL(sort_scatter_kernel, dim3(p.blocks + extra), dim3(SORT_NT), SORT_WAVES * bins * 4, s, src_rows, src_keys, src_pos,
                            n, n_rows, pass * p.bits, p.bits, p.wave_keys, w.hist, w.totals, w.keys[pass & 1], w.pos[pass & 1], p.blocks, fill);
         VDB_HIP(hipGetLastError());
     }
