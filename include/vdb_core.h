@@ -423,7 +423,7 @@ int vdb_topk_merge_keyed_strided_dev(const float* d_dist, const int64_t* d_key, 
  * where it is said.  Values are fp32, bf16 or fp16 (vdb_value_type); products and sums are taken in 32 bits or
  * more and rounded once.  Rows of a matrix are contiguous and `ld` elements apart (0 for an input = one row for
  * all); no alignment beyond the type's own is asked for.  Results do not depend on timing: equal inputs give equal
- * bits.  n = 0 is allowed and does nothing. */
+ * bits.  n = 0 is allowed and does nothing (a gradient of no lookups is zeros). */
 enum vdb_value_type { VDB_VALUE_F32 = 0, VDB_VALUE_BF16 = 1, VDB_VALUE_F16 = 2 };
 
 /* out[i] = scale * table[rows[i]], i < n; a row number outside [0, n_rows) (the -1 of an unfilled result slot)

@@ -255,7 +255,7 @@ __global__ void __launch_bounds__(SORT_NT) sort_scatter_kernel(const int64_t* __
 // has its place, in one launch over the whole chip: n^2 comparisons of two instructions.  8192 positions take 10 us, where the
 // 6 launches of the digits take 26 and one block that sorted in LDS took 21; at 16384 both forms are even.
 // A block takes 16 * KEYS positions, KEYS a thread, and all the keys into LDS; its 16 threads of a share go through a 64th of them.
-static constexpr int COUNT_NT = 1024, COUNT_LANES = 16, COUNT_SHARES = COUNT_NT / COUNT_LANES, COUNT_MAX = 12288;
+static constexpr int COUNT_NT = 1024, COUNT_LANES = 16, COUNT_SHARES = COUNT_NT / COUNT_LANES, COUNT_MAX = 12288;         // keys in less than 64 KB of LDS
 
 template <int KEYS>
 __global__ void __launch_bounds__(COUNT_NT) sort_count_kernel(const int64_t* __restrict__ rows, int n, int64_t n_rows, int blocks, int* __restrict__ keys_out,
@@ -709,7 +709,6 @@ static int launch_sort(const int64_t* rows, int64_t n, int64_t n_rows, const Gra
         const int per = std::min(std::max(ceil_div(n, COUNT_LANES * ctx().num_cus), 1), 3), blocks = ceil_div(n, COUNT_LANES * per);
         const int extra = fill_blocks(0, fill_end, COUNT_NT);
         auto kernel = per == 1 ? sort_count_kernel<1> : per == 2 ? sort_count_kernel<2> : sort_count_kernel<3>;
-        VDB_TRY(raise_dynamic_lds((const void*)kernel, COUNT_MAX * 4));
         hipLaunchKernelGGL(kernel, dim3(blocks + extra), dim3(COUNT_NT), (size_t)round_up64(n, 4) * 4, s, rows, (int)n, n_rows, blocks, w.keys[0], w.pos[0], fill);
         VDB_HIP(hipGetLastError());
         *keys = w.keys[0];
