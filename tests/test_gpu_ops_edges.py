@@ -1,0 +1,58 @@
+"""The operators on row tables and score rows at places that random inputs hardly reach, against their definitions in 64
+bits (oracle.ops_float64).  Tolerances as in test_gpu_ops."""
+
+import numpy as np
+import pytest
+
+from test_gpu_ops import TYPES, cuda, f64, ops, rng_for, sample_check  # noqa: F401 (ops is a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- sampling: rows at the beginning, lists beyond all pairs
+def uniforms_for(z, rows, kept):
+    """Uniform numbers in the middle of the shares that `rows` have among the rows `kept` of the scores z (temperature 1)."""
+    w = np.where(kept, np.exp(z - z.max()), 0.0)
+    reach = np.cumsum(w)
+    return ((reach[rows] - 0.5 * w[rows]) / reach[-1]).astype(np.float32)
+
+
+@pytest.mark.parametrize("vocab", [4097, 5002, 30522, 50257, 100277])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_sample_draws_of_the_first_rows(ops, vocab, kind):  # noqa: F811
+    """Each of the first 64 rows drawn out of lists of 300 to 1500."""
+    rng = rng_for("first rows", vocab, kind)
+    z = -12 + rng.rand(vocab)
+    z[rng.permutation(np.arange(64, vocab))[:1400]] = 2 * rng.rand(1400)
+    z[:64] = 2.2 + 0.5 * rng.rand(64)                      # the best: they remain whatever the setting
+    scores = cuda(z[None].astype(np.float32), TYPES[kind])
+    z = f64(scores)[0]
+    order = np.argsort(-z, kind="stable")
+    rows = np.arange(64)
+    for kw, keep in (({"top_k": 300}, 300), ({"top_k": 1000}, 1000), ({"min_p": 0.03}, 1464)):
+        kept = np.zeros(vocab, bool)
+        kept[order[:keep]] = True
+        got = sample_check(ops, scores.expand(64, vocab), uniforms_for(z, rows, kept), **kw)
+        assert np.array_equal(got, rows)
+
+
+@pytest.mark.parametrize("vocab", [4097, 30522, 50257])
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_sample_ties_of_the_first_rows(ops, vocab, kind):  # noqa: F811
+    """A border among the first rows, which share a score: by top-k and top-p in a list, by top-p alone."""
+    rng = rng_for("first ties", vocab, kind)
+    z = -9 + rng.rand(vocab)
+    z[rng.permutation(np.arange(200, vocab))[:280]] = 1.5 + rng.rand(280)
+    z[:100] = 1.0
+    scores = cuda(z[None].astype(np.float32), TYPES[kind])
+    z = f64(scores)[0]
+    w = np.exp(z - z.max())
+    high, tie = w[z > 1].sum(), w[0]
+    ties = np.repeat([1, 2, 7, 33, 64, 99], 4)              # how many of the equal ones remain
+    n = len(ties)
+    u = np.tile([0.0, 0.1, 0.6, 1 - 2.0 ** -24], n // 4).astype(np.float32)
+    scores = scores.expand(n, vocab)
+    sample_check(ops, scores, u, top_k=(280 + ties).astype(np.int32))
+    listed = np.full(n, 380, np.int32)
+    sample_check(ops, scores, u, top_k=listed, top_p=((high + (ties - 0.5) * tie) / (high + 100 * tie)).astype(np.float32))
+    sample_check(ops, scores, u, top_p=((high + (ties - 0.5) * tie) / w.sum()).astype(np.float32))

@@ -300,24 +300,47 @@ template <int NT> __device__ __forceinline__ void find_bin(SampleShared& sh, u64
     __syncthreads();
 }
 
+// Keys [first, last] in parts of 2^shift, at most BINS of them; the last part ends with the range.
+struct KeyRange {
+    uint32_t first, last;
+    __host__ __device__ constexpr int part_shift() const {
+        int shift = 0;
+        while ((last - first) >> shift >= (uint32_t)BINS) ++shift;
+        return shift;
+    }
+    __host__ __device__ constexpr KeyRange part(uint32_t b, int shift) const {
+        // compared before it is added: row numbers are searched as ~row, whose last part lies next to 2^32
+        const uint32_t lo = first + (b << shift), width = (1u << shift) - 1;
+        return {lo, last - lo > width ? lo + width : last};
+    }
+};
+constexpr bool parts_cover(KeyRange r) {
+    const int shift = r.part_shift();
+    const uint32_t most = (r.last - r.first) >> shift;
+    const KeyRange begin = r.part(0, shift), end = r.part(most, shift);
+    return most < (uint32_t)BINS && begin.first == r.first && (most == 0 || r.part(most - 1, shift).last == end.first - 1) && end.first <= end.last && end.last == r.last;
+}
+static_assert(parts_cover({~1u, ~0u}) && parts_cover({~4097u, ~0u}) && parts_cover({~50257u, ~0u}) && parts_cover({~131072u, ~0u}) &&
+              parts_cover({~(1u << 24), ~0u}) && parts_cover({0u, ~0u}) && parts_cover({7u, 7u}) && parts_cover({0x007fffffu, 0xff800000u}), "parts of a key range");
+
 // 11 bits of a search: the part of [*lo, *hi] in which the running sum of the weights, by descending key and from *above,
 // reaches target (false: it does not; nothing changes).  each calls f(key, weight), weight a function.
 template <int NT, class Each>
 __device__ __forceinline__ bool narrow_step(SampleShared& sh, Each&& each, uint32_t* lo, uint32_t* hi, u64* above, u64 target) {
-    const uint32_t first = *lo, last = *hi;
-    const int shift = max(21 - __clz(last - first), 0);
+    const KeyRange range{*lo, *hi};
+    const int shift = max(21 - __clz(range.last - range.first), 0);            // part_shift() at once: 21 = 32 - log2 BINS
     clear_bins<NT>(sh);
     each([&](uint32_t key, auto&& weight) {
-        if (key < first || key > last) return;
+        if (key < range.first || key > range.last) return;
         const u64 v = weight();
-        if (v) atomicAdd(&sh.bin[(key - first) >> shift], v);
+        if (v) atomicAdd(&sh.bin[(key - range.first) >> shift], v);
     });
     find_bin<NT>(sh, *above, target, true);
     if (sh.found == BINS) return false;
-    const uint32_t b = BINS - 1 - sh.found, end = first + ((b + 1) << shift) - 1;
+    const KeyRange part = range.part(BINS - 1 - sh.found, shift);
     *above = sh.found_sum;
-    *lo = first + (b << shift);
-    if (end < last) *hi = end;
+    *lo = part.first;
+    *hi = part.last;
     return true;
 }
 // The key among those of each(f) in [lo, hi] at which the running sum of the weights, by descending key and from `above`,
