@@ -477,10 +477,11 @@ int vdb_distill_step_dev(const void* d_scores, int type, int64_t n, int64_t voca
  *   min_p > 0                   of those, each with w_v >= min(min_p, 1)
  * and the draw is the first remaining row, in ascending row number, at which the running sum of the weights exceeds
  * uniform * total (the last remaining one with a weight, should none).  Where z holds +inf, those rows have weight 1 and the others none.
- * Weights are added as multiples of 2^-s, s = min(52, 62 - ceil(log2 vocab)), so sums are exact and borders do not
- * depend on the order of summation.  out_row = -1 and out_logp = -inf where nothing can be drawn; out_logp (may be
- * NULL) is the log of the drawn row's share of the remaining weights.  Settings come per row (device arrays, where
- * given) or as one value for all.  mask: packed words as everywhere (bit v % 32 of word v / 32 set = may be drawn),
+ * Weights are rounded to multiples of 2^-s, s = min(52, 62 - ceil(log2 vocab)) (2^-45 at 131072 scores; beyond 2^22
+ * scores a weight below 2^-(s+1) counts as nothing), and their sums are exact: borders do not depend on the order of
+ * summation, and lie within vocab * 2^-(s+1) of those of unrounded weights.  out_row = -1 and out_logp = -inf where
+ * nothing can be drawn; out_logp (may be NULL) is log(w / sum of the remaining weights) of the drawn row, its own w
+ * not rounded.  Settings come per row (device arrays, where given) or as one value for all.  mask: packed words as everywhere (bit v % 32 of word v / 32 set = may be drawn),
  * rows `mask_ld` words apart, 0 = one mask for all; NULL = no mask.  smaller_first != 0: the scores are distances
  * (z = -score).  vocab <= 2^24.  With a top_k, rows of up to 32768 scores need no workspace whatever the size named. */
 int vdb_sample_workspace(int64_t n, int64_t vocab, int64_t* bytes);

@@ -56,3 +56,16 @@ def test_sample_ties_of_the_first_rows(ops, vocab, kind):  # noqa: F811
     listed = np.full(n, 380, np.int32)
     sample_check(ops, scores, u, top_k=listed, top_p=((high + (ties - 0.5) * tie) / (high + 100 * tie)).astype(np.float32))
     sample_check(ops, scores, u, top_p=((high + (ties - 0.5) * tie) / w.sum()).astype(np.float32))
+
+
+@pytest.mark.parametrize("vocab", [20, 5000, 131072])
+def test_sample_logp_of_unlikely_rows(ops, vocab):  # noqa: F811
+    """The log-probability of a row far below the best is rounded to float32 and not to the steps of the sums."""
+    n = 30
+    z = np.full((n, vocab), -100.0)
+    z[:, 0] = -0.9 * (np.arange(n) + 1) + 1 / 3             # down to 2^-38.5 of the best
+    z[:, 7] = 0.0
+    z[:, 11] = -0.5
+    for kw in ({}, {"top_k": 3}, {"temperature": 0.97, "top_p": 1.0, "min_p": 0.0}):
+        got = sample_check(ops, cuda(z.astype(np.float32)), np.zeros(n, np.float32), **kw)
+        assert (got == 0).all()

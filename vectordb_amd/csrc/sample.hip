@@ -428,9 +428,10 @@ template <int NT> __device__ __forceinline__ void block_range(SampleShared& sh, 
     }
 }
 
-__device__ __forceinline__ void write_draw(const SampleArgs& a, int64_t row, uint32_t at, u64 w, u64 total) {
+// The log-probability of score z comes from the score: a weight near the cut holds few bits (ten of 2^-35 at 131072 scores).
+__device__ __forceinline__ void write_draw(const SampleArgs& a, int64_t row, uint32_t at, float z, float tau, const FixedExp& weigh, u64 total) {
     a.out_row[row] = at;
-    if (a.out_logp) a.out_logp[row] = (float)log((double)w / (double)total);
+    if (a.out_logp) a.out_logp[row] = (float)(((double)z - weigh.best) / (double)tau - log((double)total / (double)((u64)1 << a.shift)));
 }
 __device__ __forceinline__ void write_certain(const SampleArgs& a, int64_t row, int64_t at) {
     a.out_row[row] = at;
@@ -500,7 +501,7 @@ template <int NT> __device__ __forceinline__ void draw_listed(SampleShared& sh, 
             if (before) atomicAdd(&sh.pair_sum[i], before);
         }
         __syncthreads();
-        if (tid < listed && w && sh.pair_sum[tid] < least && sh.pair_sum[tid] + w >= least) write_draw(a, row, at, w, all);
+        if (tid < listed && w && sh.pair_sum[tid] < least && sh.pair_sum[tid] + w >= least) write_draw(a, row, at, zi, set.tau, weigh, all);
         return;
     }
     make_table<NT>(sh.table);
@@ -574,7 +575,7 @@ template <int NT> __device__ __forceinline__ void draw_listed(SampleShared& sh, 
     }, ~(uint32_t)a.vocab, 0xffffffffu, 0, set.goal(all), &before);
 #pragma unroll
     for (int q = 0; q < LIST_ITEMS; ++q)
-        if (w[q] && at[q] == drawn) write_draw(a, row, drawn, w[q], all);
+        if (w[q] && at[q] == drawn) write_draw(a, row, drawn, z[q], set.tau, weigh, all);
 }
 
 // ---------------------------------------------------------------- a row by one block
@@ -861,7 +862,7 @@ template <class T> __device__ __forceinline__ void sample_whole_row(SampleShared
             u64 k = run + inc - sum;
 #pragma unroll
             for (int e = 0; e < N; ++e) {
-                if (k < least && k + w[e] >= least) write_draw(a, row, (uint32_t)(at + e), w[e], total);
+                if (k < least && k + w[e] >= least) write_draw(a, row, (uint32_t)(at + e), v.get(e), set.tau, weigh, total);
                 k += w[e];
             }
             run += last_lane(inc);
@@ -1213,7 +1214,7 @@ __global__ void __launch_bounds__(FEW_NT) sample_pick_kernel(const T* __restrict
 // The row's parts, of `total` after scan_parts: the one that holds the goal, read again by the first wave.
 template <class T, class Weight>
 __device__ __forceinline__ void draw_from_parts(SampleShared& sh, const Source<T>& src, const SampleArgs& a, const SampleWork& work, int64_t row,
-                                                const Settings& set, u64 total, Weight&& weight_at) {
+                                                const Settings& set, const FixedExp& weigh, u64 total, Weight&& weight_at) {
     constexpr int N = Piece<T>::N;
     const int tid = threadIdx.x, lane = tid & 63;
     const u64 least = set.goal(total);
@@ -1239,7 +1240,7 @@ __device__ __forceinline__ void draw_from_parts(SampleShared& sh, const Source<T
         u64 k = run + inc - sum;
 #pragma unroll
         for (int e = 0; e < N; ++e) {
-            if (k < least && k + w[e] >= least) write_draw(a, row, (uint32_t)(at + e), w[e], total);
+            if (k < least && k + w[e] >= least) write_draw(a, row, (uint32_t)(at + e), v.get(e), set.tau, weigh, total);
             k += w[e];
         }
         run += last_lane(inc);
@@ -1272,7 +1273,7 @@ template <class T> __global__ void __launch_bounds__(FEW_NT) sample_border_kerne
     make_table<FEW_NT>(sh.table);
     const u64 total = scan_parts<FEW_NT>(sh, work.parts), least_w = set.least_weight(a.shift);
     const FixedExp weigh(best, set.tau, a.shift, sh.table);
-    draw_from_parts(sh, Source<T>(scores, a, row), a, work, row, set, total, [&](float z, uint32_t) {
+    draw_from_parts(sh, Source<T>(scores, a, row), a, work, row, set, weigh, total, [&](float z, uint32_t) {
         const u64 w = weigh(z);
         return w >= least_w ? w : (u64)0;
     });
@@ -1322,7 +1323,7 @@ template <class T> __global__ void __launch_bounds__(ROW_NT) sample_rest_kernel(
         if (w) atomicAdd(&sh.part[sh.list_at[i] / (uint32_t)work.part_len], w);
     }
     const u64 total = scan_parts<FEW_NT>(sh, work.parts);
-    draw_from_parts(sh, src, a, work, row, set, total, weight_at);
+    draw_from_parts(sh, src, a, work, row, set, weigh, total, weight_at);
 }
 
 // Short rows go to one block each: what the other form saves in passes it loses in launches.  Rows of 32768 scores, by one
