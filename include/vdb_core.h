@@ -430,7 +430,9 @@ enum vdb_value_type { VDB_VALUE_F32 = 0, VDB_VALUE_BF16 = 1, VDB_VALUE_F16 = 2 }
  * gives a row of zeros.  n_rows and n below 2^31. */
 int vdb_lookup_dev(const void* d_table, int table_type, int64_t n_rows, int dim, int64_t ld, const int64_t* d_rows, int64_t n,
                    float scale, void* d_out, int out_type, int64_t ld_out, void* stream);
-/* the same from the rows resident in a handle (fp32 or bf16 storage) */
+/* the same from the rows resident in a handle (fp32 or bf16 storage).  Before a handle that has been looked up in gives its
+ * rows' memory back (destroyed, or grown so that they move) it waits for the device.  A captured call reads the rows
+ * where they lay when it was captured: keep the handle and do not let it grow while the graph is in use. */
 int vdb_rows_lookup_dev(vdb_rows* h, const int64_t* d_rows, int64_t n, float scale, void* d_out, int out_type, int64_t ld_out,
                         void* stream);
 /* Gradient of a lookup: table_grad[r] = scale * sum of grad[i] over the i with rows[i] == r, zero for rows nobody

@@ -3,6 +3,7 @@ bits (oracle.ops_float64).  Tolerances as in test_gpu_ops."""
 
 import numpy as np
 import pytest
+import torch
 
 from test_gpu_ops import TYPES, cuda, f64, ops, rng_for, sample_check  # noqa: F401 (ops is a fixture)
 
@@ -69,3 +70,40 @@ def test_sample_logp_of_unlikely_rows(ops, vocab):  # noqa: F811
     for kw in ({}, {"top_k": 3}, {"temperature": 0.97, "top_p": 1.0, "min_p": 0.0}):
         got = sample_check(ops, cuda(z.astype(np.float32)), np.zeros(n, np.float32), **kw)
         assert (got == 0).all()
+
+
+# ---------------------------------------------------------------- lookups in a store
+@pytest.mark.parametrize("storage", ["f32", "bf16"])
+@pytest.mark.parametrize("end", ["close", "grow"])
+def test_store_waits_for_lookups(ops, storage, end):  # noqa: F811
+    """A store that gives its rows' memory back, because it is closed or its rows move, first waits for the lookups that read it,
+    on whatever streams they are."""
+    from vectordb_amd import _native
+    x = rng_for("store", storage).randn(3000, 64).astype(np.float32)
+    kept = cuda(x) if storage == "f32" else cuda(x).bfloat16().float()
+    a = torch.randn(4096, 4096, device="cuda")
+    rows = torch.arange(3000, device="cuda").repeat(20)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream(), torch.cuda.Stream()]
+    for s in streams:                                      # libraries and streams made ready beforehand
+        with torch.cuda.stream(s):
+            a @ a
+    store = _native.RowStore(64, storage=storage)
+    store.append(x)
+    torch.cuda.synchronize()
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            b = a
+            for _ in range(40):                            # some milliseconds of work before the lookup
+                b = b @ a
+            got.append(ops.lookup(store, rows, scale=0.5))
+    if end == "close":
+        store.close()
+    else:
+        store.append(np.zeros((200_000, 64), np.float32))
+    done = [s.query() for s in streams]
+    torch.cuda.synchronize()
+    assert all(done)
+    for g in got:
+        assert torch.equal(g, 0.5 * kept[rows])
+    store.close()

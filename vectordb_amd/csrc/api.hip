@@ -333,11 +333,19 @@ struct vdb_rows : Handle {
     bool last_used_queue = false;       // diagnostics of the last flat search
     hipStream_t last_stream = nullptr;
     const int* last_flag = nullptr;     // overflow flag of that search (device)
+    bool looked_up = false;             // lookups may still read the rows, on any streams of the caller's
+    // before the rows' memory is given back
+    int settle_lookups() {
+        if (looked_up) VDB_HIP(hipDeviceSynchronize());
+        looked_up = false;
+        return VDB_OK;
+    }
 };
 
 static int rows_reserve(vdb_rows* h, int64_t n_total, hipStream_t s) {
     Rows& r = h->r;
     if (n_total <= r.cap) return VDB_OK;
+    VDB_TRY(h->settle_lookups());
     int64_t cap = std::max<int64_t>(n_total, r.cap + r.cap / 2);
     // a 256-row chunk that starts at any stored row stays readable: the scans read whole chunks and drop what
     // lies past the end of a list or of the store
@@ -1270,6 +1278,7 @@ int vdb_rows_destroy(vdb_rows* h) {
         // work on this handle may still be queued on its own stream or, from a *_dev call, on the caller's
         (void)hipStreamSynchronize(h->stream);
         if (h->last_stream && h->last_stream != h->stream) (void)hipStreamSynchronize(h->last_stream);
+        (void)h->settle_lookups();
         h->data.release(); h->data16.release(); h->sq.release(); h->nrm.release(); h->ws.release();
         h->shadow16.release(); h->max_nrm.release(); h->slack.release();
     }
@@ -1348,6 +1357,7 @@ int vdb_rows_lookup_dev(vdb_rows* h, const int64_t* d_rows, int64_t n, float sca
     VDB_REQUIRE(h, "bad arguments to vdb_rows_lookup_dev");
     Entry g(h);
     const Rows& r = h->r;
+    if (n > 0) h->looked_up = true;
     return vdb_lookup_dev(r.bf16 ? (const void*)r.data16 : (const void*)r.data, r.bf16 ? VDB_VALUE_BF16 : VDB_VALUE_F32, r.n, r.dim,
                           r.bf16 ? r.ld16 : r.ld, d_rows, n, scale, d_out, out_type, ld_out, stream);
 }
