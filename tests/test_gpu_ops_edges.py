@@ -107,3 +107,20 @@ def test_store_waits_for_lookups(ops, storage, end):  # noqa: F811
     for g in got:
         assert torch.equal(g, 0.5 * kept[rows])
     store.close()
+
+
+# ---------------------------------------------------------------- gradient of a lookup: tables as large as are allowed
+def test_lookup_grad_largest_tables(ops):  # noqa: F811
+    """More table rows to zero than a launch holds threads for, with no positions and with more than a quarter as many."""
+    n_rows = 2 ** 30 - 1
+    out = torch.full((n_rows, 1), 7.0, device="cuda", dtype=torch.bfloat16)
+    none = torch.zeros(0, device="cuda", dtype=torch.int64)
+    ops.lookup_grad(torch.zeros(0, 1, device="cuda", dtype=torch.bfloat16), none, n_rows, out=out)
+    assert int((out != 0).sum()) == 0
+    n = 2 ** 28 + 7
+    out.fill_(7.0)
+    rows = torch.arange(n, device="cuda") * 3 + 5            # every third row once, from the sixth on
+    ops.lookup_grad(torch.ones(1, 1, device="cuda", dtype=torch.bfloat16).expand(n, 1), rows, n_rows, scale=3.0, out=out)
+    named = torch.zeros(n_rows, device="cuda", dtype=torch.bool)
+    named[rows] = True
+    assert int((out[:, 0] != 3.0 * named).sum()) == 0

@@ -392,17 +392,19 @@ template <class T> __device__ __forceinline__ void drop_neighbours(int skip, Pie
 // Blocks below zero_from: a group of 1 << log_tpr threads takes the chunk g of sorted positions; columns in slices of
 // blockIdx.y.  A row that neither starts before the chunk nor goes on behind it is finished here; the part of a row that
 // started before goes to part[g][0], of one that starts here and goes on to part[g][1].
-// The other blocks write zeros to those of zero_each table rows that no position names (slice 0 alone).
+// The other blocks write zeros to those of zero_each table rows that no position names (slice 0 alone).  A launch takes the blocks
+// from block0 on.
 template <class Tg, class To>
 __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ grad, int64_t ld, const int* __restrict__ keys,
                                                       const int* __restrict__ pos, int64_t n, float scale, To* __restrict__ out,
                                                       int64_t n_rows, int dim, int64_t ld_out, int accumulate, float* __restrict__ part,
-                                                      int chunk, int64_t chunks, int log_tpr, int zero_from, int log_zero, int zero_each) {
-    if ((int)blockIdx.x >= zero_from) {
+                                                      int chunk, int64_t chunks, int log_tpr, int block0, int zero_from, int log_zero, int zero_each) {
+    const int block = block0 + (int)blockIdx.x;
+    if (block >= zero_from) {
         if (blockIdx.y) return;
         __shared__ int64_t range[2];
         __shared__ int named[ZERO_ROWS];
-        const int64_t r0 = (int64_t)((int)blockIdx.x - zero_from) * zero_each;
+        const int64_t r0 = (int64_t)(block - zero_from) * zero_each;
         if (threadIdx.x < ZERO_ROWS) named[threadIdx.x] = 0;
         if (threadIdx.x < 128) {
             const int64_t at = lower_bound_wave(keys, n, r0 + (threadIdx.x >> 6) * zero_each);
@@ -426,7 +428,7 @@ __global__ void __launch_bounds__(256) seg_sum_kernel(const Tg* __restrict__ gra
         return;
     }
     constexpr int N = Piece<Tg>::N;
-    const int64_t g = (int64_t)blockIdx.x * (256 >> log_tpr) + (threadIdx.x >> log_tpr);
+    const int64_t g = (int64_t)block * (256 >> log_tpr) + (threadIdx.x >> log_tpr);
     const int c = ((blockIdx.y << log_tpr) + (threadIdx.x & ((1 << log_tpr) - 1))) * N;
     if (g >= chunks || c >= dim) return;
     const int64_t p0 = g * chunk, p1 = min(p0 + chunk, n);
@@ -776,9 +778,13 @@ static int launch_lookup_grad(const void* grad, int grad_type, int64_t ld, const
             // two blocks a CU for the zeros of small tables (1963 x 469 bf16 into 4316 rows: 22 us with 64 rows each, so 18)
             const int zero_each = (int)std::min<int64_t>(std::max<int64_t>(n_rows / (2 * ctx().num_cus), 8), ZERO_ROWS);
             const int sums = ceil_div(chunks, 256 >> l), zeros = accumulate || filled ? 0 : ceil_div(n_rows, zero_each);
-            hipLaunchKernelGGL((seg_sum_kernel<Tg, To>), dim3(sums + zeros, ceil_div(pieces, 1 << l)), dim3(256), 0, s, (const Tg*)grad, ld, keys, pos,
-                               n, scale, (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks, l, sums, lz, zero_each);
-            VDB_HIP(hipGetLastError());
+            const int most = 1 << 23;                                      // a launch holds fewer than 2^32 threads
+            for (int block0 = 0; block0 < sums + zeros; block0 += most) {
+                hipLaunchKernelGGL((seg_sum_kernel<Tg, To>), dim3(std::min(sums + zeros - block0, most), ceil_div(pieces, 1 << l)), dim3(256), 0, s,
+                                   (const Tg*)grad, ld, keys, pos, n, scale, (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks, l, block0,
+                                   sums, lz, zero_each);
+                VDB_HIP(hipGetLastError());
+            }
             if (chunks > 1) {
                 hipLaunchKernelGGL((seg_join_kernel<To>), dim3(ceil_div(chunks - 1, JOIN_CHUNKS), ceil_div(dim, 256)), dim3(JOIN_NT), 0, s, keys, n, scale,
                                    (To*)out, n_rows, dim, ld_out, accumulate, w.part, chunk, chunks);
@@ -809,7 +815,7 @@ int vdb_lookup_dev(const void* d_table, int table_type, int64_t n_rows, int dim,
 }
 
 static int check_grad_sizes(int64_t n, int64_t n_rows, int dim) {
-    // what the grids of its launches hold
+    // what the sort's 32-bit keys, positions and counts hold
     const int64_t most = (int64_t)1 << 30;
     VDB_REQUIRE(n >= 0 && n < most && n_rows >= 0 && n_rows < most && dim >= 1 && dim <= 1 << 23,
                 "bad sizes for a lookup gradient: %lld rows into %lld, dimension %d", (long long)n, (long long)n_rows, dim);
