@@ -13,9 +13,10 @@ row) slots with row -1 where there is nothing; the filters of ``sample`` are the
 
 Every function enqueues on the current torch stream and returns without waiting; inputs made on another stream have to
 be ordered by the caller, as for any torch operation.  Nothing is allocated but the outputs (or none, with ``out=``) and a
-workspace from torch's allocator, so the calls can be captured into a graph.  Autograd does not see them: gradients are
-the functions named ``*_grad``, which a ``torch.autograd.Function`` can call.  An ``out`` shares no memory with the inputs but
-where it is said.  Values are float32, bfloat16 or float16, sums
+workspace from torch's allocator, so the calls can be captured into a graph.  Autograd does not record them: gradients are
+the functions named ``*_grad``, which a ``torch.autograd.Function`` calls, and a tensor that requires a gradient is refused
+where gradients are recorded (so call them under ``torch.no_grad()`` or in such a function).  An ``out`` shares no memory with the
+inputs but where it is said.  Values are float32, bfloat16 or float16, sums
 are taken in 32 bits or more, and equal inputs give equal bits.  Arguments that do not fit raise ``ValueError``.
 """
 
@@ -52,12 +53,16 @@ def _start() -> None:
 def _on_gpu(t, what: str) -> None:
     if not isinstance(t, torch.Tensor):
         _fail(f"{what} must be a torch tensor, got {type(t).__name__}")
-    if not t.is_cuda:
-        _fail(f"{what} must be on the GPU, it is on {t.device}")
-    if _lib is None:
-        _start()
-    if t.get_device() != _device_no:
-        _fail(f"{what} must be on GPU {_device_no}, the library's device; it is on {t.device}")
+    if t.requires_grad and torch.is_grad_enabled():
+        _fail(f"{what} requires a gradient, which this call would not record: call it under torch.no_grad() or in a torch.autograd.Function, "
+              f"with the *_grad functions for the gradients")
+    if _lib is None or t.get_device() != _device_no:
+        if not t.is_cuda:
+            _fail(f"{what} must be on the GPU, it is on {t.device}")
+        if _lib is None:
+            _start()
+        if t.get_device() != _device_no:
+            _fail(f"{what} must be on GPU {_device_no}, the library's device; it is on {t.device}")
 
 
 def _matrix(t, what: str) -> Tuple[int, int, int, int]:
