@@ -1,4 +1,4 @@
-"""vectordb_amd.ops and autograd: gradients are not lost in silence."""
+"""vectordb_amd.ops and autograd: gradients are not lost in silence, and what is written in place is noticed."""
 
 import pytest
 import torch
@@ -64,3 +64,23 @@ def test_gradients_of_a_function(native):
     (Rows.apply(table, at) * weight).sum().backward()
     want = torch.zeros(30, 8, device="cuda").index_add_(0, at, 0.5 * weight)
     assert torch.equal(table.grad, want)                   # multiples of 1/2: exact
+
+
+@pytest.mark.gpu
+def test_writing_to_out_is_noticed(native):
+    """A tensor that autograd has kept, overwritten by a call, makes the backward pass fail as after any in-place operation."""
+    for call, args, names in arguments("cuda"):
+        if "out" not in args:
+            continue
+        factor = torch.ones_like(args["out"], requires_grad=True)
+        kept = (factor * args["out"]).sum()
+        call(**args)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            kept.backward()
+    x = torch.zeros(4, 8, device="cuda")
+    factor = torch.ones_like(x, requires_grad=True)
+    kept = (factor * x).sum()
+    call, args, _ = arguments("cuda")[4]
+    call(**{**args, "scores": x, "out": x})                # in place of the scores
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        kept.backward()

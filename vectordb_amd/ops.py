@@ -16,7 +16,7 @@ be ordered by the caller, as for any torch operation.  Nothing is allocated but 
 workspace from torch's allocator, so the calls can be captured into a graph.  Autograd does not record them: gradients are
 the functions named ``*_grad``, which a ``torch.autograd.Function`` calls, and a tensor that requires a gradient is refused
 where gradients are recorded (so call them under ``torch.no_grad()`` or in such a function).  An ``out`` shares no memory with the
-inputs but where it is said.  Values are float32, bfloat16 or float16, sums
+inputs but where it is said; writing to it counts as an in-place change of that tensor.  Values are float32, bfloat16 or float16, sums
 are taken in 32 bits or more, and equal inputs give equal bits.  Arguments that do not fit raise ``ValueError``.
 """
 
@@ -105,6 +105,12 @@ def _output(out, what: str, shape, dtype: torch.dtype) -> torch.Tensor:
     return out
 
 
+def _written(given: Optional[torch.Tensor]) -> None:
+    """What was written to a caller's tensor is seen by autograd, which may have kept it for a backward pass."""
+    if given is not None:
+        torch.autograd.graph.increment_version(given)
+
+
 def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
@@ -154,7 +160,7 @@ def lookup(table: Union[torch.Tensor, "_native.RowStore"], rows: torch.Tensor, s
     if dtype not in VALUE_TYPES:
         _fail(f"dtype must be float32, bfloat16 or float16, got {dtype}")
     shape = tuple(rows.shape) + (dim,)
-    out = _output(out, "out", shape, dtype)
+    given, out = out, _output(out, "out", shape, dtype)
     if out.dim() != 2 and not out.is_contiguous():
         _fail("out must be contiguous unless rows is a vector")
     ld_out = out.stride(0) if out.dim() == 2 and n > 1 else dim
@@ -162,6 +168,7 @@ def lookup(table: Union[torch.Tensor, "_native.RowStore"], rows: torch.Tensor, s
         _native.check(_lib.vdb_rows_lookup_dev(store.h, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], ld_out, _stream()))
     else:
         _native.check(_lib.vdb_lookup_dev(_p(table), code, n_rows, dim, ld, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], ld_out, _stream()))
+    _written(given)
     return out
 
 
@@ -186,10 +193,11 @@ def lookup_grad(grad: torch.Tensor, rows: torch.Tensor, n_rows: int, scale: floa
     dtype = dtype or (out.dtype if out is not None else grad.dtype)
     if dtype not in VALUE_TYPES:
         _fail(f"dtype must be float32, bfloat16 or float16, got {dtype}")
-    out = _output(out, "out", (n_rows, dim), dtype)
+    given, out = out, _output(out, "out", (n_rows, dim), dtype)
     keep, work, size = _workspace("vdb_lookup_grad_workspace", n, n_rows, dim)
     _native.check(_lib.vdb_lookup_grad_dev(_p(grad), code, ld, _p(rows), n, scale, _p(out), VALUE_TYPES[dtype], n_rows, dim,
                                                      out.stride(0) if n_rows > 1 else dim, int(accumulate), work, size, _stream()))
+    _written(given)
     return out
 
 
@@ -242,8 +250,9 @@ def distill_grad(scores: torch.Tensor, teacher: torch.Tensor, rows: torch.Tensor
     if stats.dtype != torch.float32 or tuple(stats.shape) != (n, 2) or not stats.is_contiguous():
         _fail(f"stats must be contiguous float32 of shape ({n}, 2), got {stats.dtype} of shape {tuple(stats.shape)}")
     _vector(grad_loss, "grad_loss", n, torch.float32)
-    out = _output(out, "out", (n, vocab), scores.dtype)
+    given, out = out, _output(out, "out", (n, vocab), scores.dtype)
     _native.check(_lib.vdb_distill_grad_dev(*args, _p(stats), _p(grad_loss), _p(out), out.stride(0) if n > 1 else vocab, _stream()))
+    _written(given)
     return out
 
 
@@ -254,10 +263,11 @@ def distill_step(scores: torch.Tensor, teacher: torch.Tensor, rows: torch.Tensor
     n, vocab = scores.shape
     _vector(grad_loss, "grad_loss", n, torch.float32)
     loss = torch.empty(n, device=_where, dtype=torch.float32)
-    out = _output(out, "out", (n, vocab), scores.dtype)
+    given, out = out, _output(out, "out", (n, vocab), scores.dtype)
     keep, work, size = _workspace("vdb_distill_workspace", n, vocab)
     _native.check(_lib.vdb_distill_step_dev(*args, _p(grad_loss), _p(loss), None, _p(out), out.stride(0) if n > 1 else vocab,
                                                       work, size, _stream()))
+    _written(given)
     return loss, out
 
 
