@@ -451,11 +451,13 @@ int vdb_lookup_grad_dev(const void* d_grad, int grad_type, int64_t ld, const int
  *         row where that is given (the teacher's mass outside the list is then left out)
  *   loss = tau^2 * sum_j p_j (log p_j - log q_{r_j})
  *   d loss / d z_v = tau * (sum_j p_j * q_v - sum of p_j with r_j == v)
- * A slot with a row number outside [0, vocab) or a score of -inf is unfilled; a row without filled slots has loss
- * and gradient 0 whatever its scores are.  stats, where wanted, takes (max z, log sum_v exp((z_v - max z) / tau)) of every
+ * Larger scores are better: a search's distances are negated, the student's scores as well where they are distances.
+ * A slot with a row number outside [0, vocab) or a score of -inf is unfilled; a row without filled slots, or whose p_j
+ * are all 0, has loss and gradient 0 whatever its scores are.  stats, where wanted, takes (max z, log sum_v exp((z_v - max z) / tau)) of every
  * row: what the gradient needs of the forward pass.  Scores of -inf have q = 0 (and loss +inf where the teacher names
  * one); a row that holds a NaN or +inf has a NaN loss and gradient, other rows are not affected.  temperature lies in
- * [1e-6, 1e6].
+ * [1e-6, 1e6]; the loss is tau^2 times a difference of fp32 logarithms, each rounded to 2^-24 of itself, so where tau is large
+ * and the two distributions are close, less of it is left.
  * The gradient of row i is scaled by grad_loss[i] (0 = zeros whatever the row holds); d_grad may be d_scores itself
  * (same ld), otherwise the two do not overlap.  vdb_distill_step_dev computes both for weights known beforehand. */
 #define VDB_DISTILL_MAX_K 1024
@@ -483,9 +485,10 @@ int vdb_distill_step_dev(const void* d_scores, int type, int64_t n, int64_t voca
  * scores a weight below 2^-(s+1) counts as nothing), and their sums are exact: borders do not depend on the order of
  * summation, and lie within vocab * 2^-(s+1) of those of unrounded weights.  out_row = -1 and out_logp = -inf where
  * nothing can be drawn; out_logp (may be NULL) is log(w / sum of the remaining weights) of the drawn row, its own w
- * not rounded.  Settings come per row (device arrays, where given) or as one value for all.  mask: packed words as everywhere (bit v % 32 of word v / 32 set = may be drawn),
- * rows `mask_ld` words apart, 0 = one mask for all; NULL = no mask.  smaller_first != 0: the scores are distances
- * (z = -score).  vocab <= 2^24.  With a top_k, rows of up to 32768 scores need no workspace whatever the size named. */
+ * not rounded.  Settings come per row (device arrays, where given) or as one value for all.  mask: packed words as
+ * everywhere (bit v % 32 of word v / 32 set = may be drawn), rows `mask_ld` words apart, 0 = one mask for all; NULL = no
+ * mask.  smaller_first != 0: the scores are distances (z = -score).  vocab <= 2^24.  With a top_k, rows of up to 32768
+ * scores need no workspace whatever the size named. */
 int vdb_sample_workspace(int64_t n, int64_t vocab, int64_t* bytes);
 int vdb_sample_dev(const void* d_scores, int type, int64_t n, int64_t vocab, int64_t ld, int smaller_first, const float* d_uniform,
                    const float* d_temperature, float temperature, const int32_t* d_top_k, int top_k, const float* d_top_p, float top_p,

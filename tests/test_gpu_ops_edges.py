@@ -5,7 +5,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_gpu_ops import TYPES, cuda, f64, ops, rng_for, sample_check  # noqa: F401 (ops is a fixture)
+from oracle import ops_float64 as R
+from test_gpu_ops import TYPES, U, cuda, f64, ops, rng_for, sample_check  # noqa: F401 (ops is a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -124,3 +125,40 @@ def test_lookup_grad_largest_tables(ops):  # noqa: F811
     named = torch.zeros(n_rows, device="cuda", dtype=torch.bool)
     named[rows] = True
     assert int((out[:, 0] != 3.0 * named).sum()) == 0
+
+
+# ---------------------------------------------------------------- sampling: long rows that neither a list nor one bin settles
+@pytest.mark.parametrize("kind", ["f32", "bf16"])
+def test_sample_rows_without_outliers(ops, kind):  # noqa: F811
+    """131072 scores of standard deviation 1: borders in the bulk, where a bin or a list is too small for those at the border."""
+    rng = rng_for("bulk", kind)
+    z = cuda(rng.randn(3, 131_072).astype(np.float32), TYPES[kind])
+    u = np.array([0.02, 0.5, 0.97], np.float32)
+    for kw in ({"temperature": 2.0, "top_p": 0.5}, {"temperature": 2.0, "top_p": 0.9}, {"temperature": 3.0, "min_p": 0.02}, {"min_p": 0.1}, {"top_k": 5000},
+               {"top_k": 1025, "top_p": 0.5}, {"top_p": 0.3, "min_p": 0.05}):
+        sample_check(ops, z, u, **kw)
+
+
+# ---------------------------------------------------------------- distillation from a search
+@pytest.mark.parametrize("n_rows", [7, 2000])
+def test_distill_from_a_search(ops, n_rows):  # noqa: F811
+    """The lists of a search as a teacher: distances, negated, with slots that a small store cannot fill."""
+    from vectordb_amd import _native
+    rng = rng_for("search", n_rows)
+    x, q, k = rng.randn(n_rows, 48).astype(np.float32), rng.randn(9, 48).astype(np.float32), 10
+    store = _native.RowStore(48)
+    store.append(x)
+    queries = cuda(q)
+    dist, rows = torch.empty(9, k, device="cuda"), torch.empty(9, k, dtype=torch.int64, device="cuda")
+    store.search_device(queries.data_ptr(), 9, k, _native.METRIC_CODES["euclidean"], dist.data_ptr(), rows.data_ptr(),
+                        stream=torch.cuda.current_stream().cuda_stream)
+    scores = torch.randn(9, n_rows, device="cuda")
+    loss, stats = ops.distill(scores, -dist, rows)
+    grad = ops.distill_grad(scores, -dist, rows, stats, torch.ones(9, device="cuda"))
+    assert bool((rows < 0).any()) == (n_rows < k)
+    for i in range(9):
+        r = R.distill_row(f64(scores[i]), f64(-dist[i]), rows[i].cpu().numpy(), 1.0)
+        # sums of 2000 / 256 terms a thread and of ten slots, exponents up to 10: 200 roundings cover them
+        assert abs(float(loss[i]) - r["loss"]) <= 200 * U * max(1.0, abs(r["loss"]))
+        assert (np.abs(f64(grad[i]) - r["grad"]) <= 200 * U * (r["q"] + r["target"])).all()
+    store.close()

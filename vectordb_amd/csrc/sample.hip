@@ -7,12 +7,16 @@
 //     the maxima of k groups or more) go to a list in LDS, in row order, and everything else happens there;
 //   - top-p alone takes a histogram of the weights over the distance from the best score, and then the scores of the one
 //     bin in which the border lies, narrowed by their ordered bit patterns.
-// Weights exp((z - max) / tau) are taken in double, to 2^-50, and added as 64-bit integers (multiples of 2^-s): sums do not
-// depend on the order in which threads add, and the draw is the one of the definition.
+// Weights exp((z - max) / tau) are taken in double, to 2^-50, rounded to multiples of 2^-s (2^-45 at 131072 scores) and added as
+// 64-bit integers: sums are exact and do not depend on the order in which threads add.  s is as large as the sum of a row of
+// weights of 1 allows; a border lies within vocab * 2^-(s+1) of that of unrounded weights, 2^-29 of the best one's weight at 131072.
 //
 // Two forms.  Short rows: a block of 1024 threads takes a row through all its passes.  Long rows are streamed by the whole
 // chip: one pass takes the maxima of groups of 32 scores (the floor: n * vocab values read once), a block per row finishes
-// the rows that a list settles from those maxima, and for the others two more passes add up weights.
+// the rows that a list settles from those maxima, and for the others two more passes add up weights.  A top-k above LIST_MAX / 2, a
+// list or a border's bin of more than LIST_MAX scores send a row through all its passes by one block, behind the passes that
+// the chip went through: of 131072 bf16 scores of standard deviation 1, one row 103 us with top-k 5000, 222 with temperature 2
+// and top-p 0.5, 256 rows 131 and 319 us (131 with top-p 0.9, whose bin is small enough).
 #include "vdb_internal.h"
 #include "values.h"
 
@@ -385,7 +389,7 @@ __device__ __forceinline__ uint32_t narrow(SampleShared& sh, Each&& each, uint32
 }
 __device__ __forceinline__ u64 one_each() { return 1; }
 // A bound that no fewer than k of the scores of each(f) reach, and few more: the lower end of the part in which the k-th
-// largest lies.  lowest, best: their range.  -LOWEST where there are fewer than k.
+// largest lies.  lowest, best: their range.  LOWEST where there are fewer than k.
 template <int NT, class Each> __device__ __forceinline__ float bound_of(SampleShared& sh, Each&& each, float lowest, float best, int k) {
     uint32_t lo = pattern(lowest), hi = pattern(best);
     u64 above = 0;

@@ -9,7 +9,8 @@ position, or a query's distances.
     sample                                 one row number drawn from each score row
 
 The reference has no counterpart.  The teacher's lists and the row numbers have the form of a search result: (score,
-row) slots with row -1 where there is nothing; the filters of ``sample`` are the packed row masks that searches take.
+row) slots with row -1 where there is nothing.  Scores are better the larger they are, so a search's distances are negated for a
+teacher's list; ``sample`` takes distances as they are with ``distances=True``.  Its filters are the packed row masks of searches.
 
 Every function enqueues on the current torch stream and returns without waiting; inputs made on another stream have to
 be ordered by the caller, as for any torch operation.  Nothing is allocated but the outputs (or none, with ``out=``) and a
@@ -17,7 +18,8 @@ workspace from torch's allocator, so the calls can be captured into a graph.  Au
 the functions named ``*_grad``, which a ``torch.autograd.Function`` calls, and a tensor that requires a gradient is refused
 where gradients are recorded (so call them under ``torch.no_grad()`` or in such a function).  An ``out`` shares no memory with the
 inputs but where it is said; writing to it counts as an in-place change of that tensor.  Values are float32, bfloat16 or float16, sums
-are taken in 32 bits or more, and equal inputs give equal bits.  Arguments that do not fit raise ``ValueError``.
+are taken in 32 bits or more, and equal inputs give equal bits.  Arguments that do not fit raise ``ValueError``.  Tensors lie on the
+library's device, which every call makes the current one of its thread.
 """
 
 from __future__ import annotations
@@ -230,7 +232,8 @@ def distill(scores: torch.Tensor, teacher: torch.Tensor, rows: torch.Tensor, tem
     With tau = ``temperature``, q = softmax(scores / tau) and p = softmax of a row's filled slots / tau, or
     exp(teacher / tau - teacher_lse) where the log-sum-exp over the teacher's whole row is given:
     ``loss = tau^2 * sum_j p_j (log p_j - log q[rows_j])``.  A row without filled slots has loss 0.  ``stats`` is what
-    ``distill_grad`` needs of this pass."""
+    ``distill_grad`` needs of this pass.  A search's distances go in negated.  The logarithms are float32: of a loss that a large
+    temperature makes a small difference of them, times tau^2, less is left."""
     args = _distill_args(scores, teacher, rows, temperature, teacher_lse)
     n, vocab = scores.shape
     loss = torch.empty(n, device=_where, dtype=torch.float32)
@@ -283,7 +286,11 @@ def sample(scores: torch.Tensor, uniforms: torch.Tensor, temperature: Union[floa
     None = off) relative to the best row.  The draw is the first remaining row, in ascending row number, at which the running
     sum of the probabilities exceeds ``uniforms`` [n] (float32 in [0, 1)).  Equal scores rank by row number.
     ``mask_words``: packed row filter, int32 or uint32 words, one per row of ``scores`` or one for all; rows whose bit is 0, scores of
-    -inf and NaN are never drawn.  ``distances``: smaller scores are better.  Where nothing can be drawn: (-1, -inf)."""
+    -inf and NaN are never drawn.  ``distances``: smaller scores are better.  Where nothing can be drawn: (-1, -inf).
+
+    Weights exp((score - best) / temperature) below 2^-40 count as nothing, and the others are summed as multiples of 2^-s, s =
+    min(52, 62 - ceil(log2 of the row's length)): sums are exact, and a border or a draw is that of weights which are off by at most
+    2^-(s+1) each (2^-46 at 131072 scores).  The log-probability is of the drawn row's own weight, not rounded."""
     code, n, vocab, ld = _matrix(scores, "scores")
     if vocab < 1:
         _fail("a score row must have at least one value")
